@@ -78,6 +78,20 @@ class CsaqP2PGroup(ctypes.Structure):
     ]
 
 
+class CsaqKvqCache(ctypes.Structure):
+    """Mirror of ``csaq_kvq_cache`` (include/csaq_b200.h)."""
+
+    _fields_ = [
+        ("k_codes", c_vp),
+        ("k_params", c_vp),
+        ("v_codes", c_vp),
+        ("v_params", c_vp),
+        ("Lmax", c_i64),
+        ("bits", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "csaq_version": (ctypes.c_char_p, []),
@@ -140,6 +154,14 @@ _SIGNATURES = {
                                              c_vp, c_vp, c_i64, ctypes.c_float, c_int, c_vp]),
     "csaq_p2p_errors": (c_int, [ctypes.POINTER(CsaqP2PGroup), ctypes.POINTER(c_i64)]),
     "csaq_p2p_set_spin_limit": (c_int, [c_i64]),
+    "csaq_kvq_write": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                               c_vp, c_i64, c_vp, ctypes.POINTER(CsaqKvqCache), c_int, c_vp]),
+    "csaq_kvq_read": (c_int, [ctypes.POINTER(CsaqKvqCache), c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int,
+                              c_vp]),
+    "csaq_kvq_attention_workspace_floats": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "csaq_kvq_attention_tickets": (c_i64, [c_i64, c_i64, c_i64, c_i64]),
+    "csaq_kvq_attention": (c_int, [c_vp, c_i64, ctypes.POINTER(CsaqKvqCache), c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
+                                   ctypes.c_float, c_vp, c_vp, c_vp, c_i64, c_int, c_vp]),
     "csaq_silu_mul": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]),
     "csaq_spec_accept": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "csaq_greedy_commit": (c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),

@@ -382,6 +382,63 @@ int csaq_decode_attention_static(const void* q, const void* k_cache, const void*
                                  const int32_t* pos0, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
                                  int64_t D, int64_t Lmax, float scale, void* out, int dtype, void* stream);
 
+/* ── Quantised KV cache ──────────────────────────────────────────────────────
+ * No counterpart in the reference (its cache is the HF module's, in the model's
+ * dtype). One layer's keys and values as 8- or 4-bit codes with one scale and
+ * zero point per (token, head, group of group_size head elements):
+ *   codes  (B, Hkv, Lmax, D * bits / 8) bytes, 4-bit: even element in the low nibble;
+ *   params (B, Hkv, Lmax, D / group_size) words: upper 16 bits the bf16 scale s,
+ *          lower 16 bits 0x6400 + zero point z.
+ * An element is s * (code - z), exact in fp32; zero is always representable. The
+ * error of a stored element is at most 1.01 s, s at most 1.01 * (largest - smallest
+ * element of its group, counting 0) / (2^bits - 1). D is 64 or 128, group_size 64
+ * or D, Lmax a multiple of 16, the four buffers 16-byte aligned (else
+ * CSAQ_ERR_UNSUPPORTED). Zeroed buffers are a cache of zeros. */
+typedef struct csaq_kvq_cache {
+  uint8_t* k_codes;
+  uint32_t* k_params;
+  uint8_t* v_codes;
+  uint32_t* v_params;
+  int64_t Lmax;
+  int32_t bits;
+  int32_t group_size;
+} csaq_kvq_cache;
+
+/* Quantise a step's keys and values into the cache at positions pos0[b] + s
+ * (rows b*S+s of k and v, Hkv*D wide, ldk/ldv elements apart). With cos_t and
+ * sin_t (n_rope rows of D fp32, the layout of csaq_rope_kv) the keys are rotated
+ * first, in fp32 without a rounding to dtype in between, and the queries q
+ * (nullable) are rotated into q_out (M, Hq, D); with both null the keys are
+ * stored as they are and q must be null. A position outside [0, Lmax) or the
+ * tables is not stored and its query passes unrotated. A group with a NaN or an
+ * infinity reads back as NaN. Needs 16-byte aligned q, k, v, q_out, tables and
+ * row strides that are multiples of 8 elements. */
+int csaq_kvq_write(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                   const int32_t* pos0, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                   const float* cos_t, const float* sin_t, int64_t n_rope, void* q_out,
+                   const csaq_kvq_cache* cache, int dtype, void* stream);
+
+/* Read positions [start, start + n) of every sequence and head back: k_out and
+ * v_out (either may be null) are (B, Hkv, n, D) contiguous in dtype (F32, F16 or
+ * BF16), 16-byte aligned. */
+int csaq_kvq_read(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D, int64_t start, int64_t n,
+                  void* k_out, void* v_out, int dtype, void* stream);
+
+/* csaq_decode_attention against a quantised cache: token (b, s), row b*S+s of q
+ * (Hq*D wide, ldq elements apart), attends keys 0 .. min(pos0[b]+s, Lmax-1); a
+ * token at a negative position sees nothing and its output is 0 (an unused
+ * sequence of a batch: pos0[b] = -S). Any S. out rows are ldo elements apart.
+ * part: csaq_kvq_attention_workspace_floats floats; tickets:
+ * csaq_kvq_attention_tickets int32, zero before the first call (calls leave them
+ * zero); calls that may overlap on the GPU need a workspace each. A token's
+ * result does not depend on S or on the other sequences. */
+int64_t csaq_kvq_attention_workspace_floats(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t Lmax);
+int64_t csaq_kvq_attention_tickets(int64_t B, int64_t S, int64_t Hq, int64_t Hkv);
+int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cache* cache, const int32_t* pos0, int64_t B,
+                       int64_t S, int64_t Hq, int64_t Hkv, int64_t D, float scale, float* part, int32_t* tickets,
+                       void* out, int64_t ldo, int dtype, void* stream);
+
 /* HF LlamaMLP gate: h = dtype(silu(g)) * u. */
 int csaq_silu_mul(const void* g, int64_t ldg, const void* u, int64_t ldu, void* h, int64_t ldh,
                   int64_t M, int64_t N, int dtype, void* stream);
