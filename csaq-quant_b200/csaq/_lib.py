@@ -92,6 +92,21 @@ class CsaqKvqCache(ctypes.Structure):
     ]
 
 
+class CsaqSampleParams(ctypes.Structure):
+    """Mirror of ``csaq_sample_params`` (include/csaq_b200.h)."""
+
+    _fields_ = [
+        ("temperature", c_vp),
+        ("top_k", c_vp),
+        ("top_p", c_vp),
+        ("min_p", c_vp),
+        ("temperature_all", ctypes.c_float),
+        ("top_k_all", ctypes.c_int32),
+        ("top_p_all", ctypes.c_float),
+        ("min_p_all", ctypes.c_float),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "csaq_version": (ctypes.c_char_p, []),
@@ -141,6 +156,8 @@ _SIGNATURES = {
     "csaq_argmax_parts": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_int, c_vp]),
     "csaq_sample_rows": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, ctypes.c_float, ctypes.c_float,
                                  ctypes.c_uint64, c_vp, c_vp, c_int, c_vp]),
+    "csaq_sample_filtered": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(CsaqSampleParams), c_vp,
+                                     c_vp, c_int, c_vp]),
     "csaq_spec_sample_verify": (c_int, [c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64,
                                         ctypes.c_float, ctypes.c_float, ctypes.c_uint64, c_vp, c_vp, c_int, c_vp]),
     "csaq_p2p_alloc": (c_int, [c_i64, ctypes.POINTER(c_vp)]),

@@ -460,6 +460,36 @@ int csaq_spec_accept(const int64_t* draft, const int64_t* verify_argmax, int64_t
 int csaq_sample_rows(const void* logits, int n_parts, int64_t part_stride, int64_t ld, int64_t part_len,
                      int64_t rows, float temperature, float top_p, uint64_t seed, uint64_t* counter, int64_t* out,
                      int dtype, void* stream);
+/* Sampling settings of csaq_sample_filtered: a device array of one value per
+ * row, or (pointer null) one value for all rows. temperature not above 0: the
+ * first rank; top_k <= 0, top_p >= 1 (or NaN) and min_p <= 0 (or NaN) are off;
+ * top_p <= 0 keeps the first rank. */
+typedef struct csaq_sample_params {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+} csaq_sample_params;
+
+/* One token per logit row from the given random number random[row] in [0, 1)
+ * (csaq_sample_rows draws its own and has temperature and top-p only). With
+ * w_j = exp((x_j - max x) / temperature) and tokens ranked by falling logit, the
+ * lower index first among equals: top-k keeps the first k ranks; top-p keeps of
+ * those the ranks whose preceding mass is at most top_p times the mass of the
+ * top-k set; min-p keeps of those the tokens with w_j >= min_p. out[row] is the
+ * first index whose cumulative kept weight, in index order, exceeds random[row]
+ * times the kept mass. Weights and sums are fp64 and their order is fixed. NaN
+ * and -inf logits are never drawn, +inf ones share the whole mass; a row of NaN
+ * and -inf gives -1. Rows are n_parts slices like csaq_sample_rows; a row of
+ * up to 270,000 fp32 or 550,000 16-bit logits (else CSAQ_ERR_UNSUPPORTED). */
+int csaq_sample_filtered(const void* logits, int n_parts, int64_t part_stride, int64_t ld, int64_t part_len,
+                         int64_t rows, const csaq_sample_params* params, const float* random, int64_t* out, int dtype,
+                         void* stream);
+
 /* vt (B x (K+1)) for csaq_spec_accept from the draft tokens (B x K), the
  * draft steps' full-vocabulary logits (K x B x V, contiguous) and the verify
  * logits (rows b*(K+1)+k): rejection sampling of each draft token, a residual
