@@ -46,7 +46,6 @@ class KVWorkspace:
     ordered on the GPU (one stream, or one captured graph replayed at a time)."""
 
     part: torch.Tensor
-    tickets: torch.Tensor
 
 
 class QuantizedKVCache:
@@ -106,6 +105,7 @@ class QuantizedKVCache:
         self.device = kc.device
         self._c = CsaqKvqCache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(), L, bits, self.group_size)
         self._ref = ctypes.byref(self._c)
+        self._sizes = {}  # (tokens, heads) -> floats of attend's scratch
 
     def buffers(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         return self.k_codes, self.k_params, self.v_codes, self.v_params
@@ -215,13 +215,18 @@ class QuantizedKVCache:
 
     def workspace(self, tokens: int, heads: int) -> KVWorkspace:
         """Scratch for ``attend`` with up to `tokens` tokens per sequence and `heads` query heads."""
-        L = lib()
-        n = L.csaq_kvq_attention_workspace_floats(self.batch, tokens, heads, self.kv_heads, self.head_dim, self.max_len)
-        t = L.csaq_kvq_attention_tickets(self.batch, tokens, heads, self.kv_heads)
-        if n < 0 or t < 0:
-            raise ValueError(f"csaq-b200: no attention of {tokens} tokens and {heads} heads over {self.kv_heads} KV heads")
-        return KVWorkspace(torch.empty(n, dtype=torch.float32, device=self.device),
-                           torch.zeros(t, dtype=torch.int32, device=self.device))
+        return KVWorkspace(torch.empty(self._floats(tokens, heads), dtype=torch.float32, device=self.device))
+
+    def _floats(self, tokens: int, heads: int) -> int:
+        n = self._sizes.get((tokens, heads))
+        if n is None:
+            n = lib().csaq_kvq_attention_workspace_floats(self.batch, tokens, heads, self.kv_heads, self.head_dim,
+                                                          self.max_len)
+            if n < 0:
+                raise ValueError(f"csaq-b200: no attention of {tokens} tokens and {heads} heads over "
+                                 f"{self.kv_heads} KV heads")
+            self._sizes[(tokens, heads)] = n
+        return n
 
     def attend(self, q: torch.Tensor, pos0: torch.Tensor, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, workspace: Optional[KVWorkspace] = None) -> torch.Tensor:
@@ -240,15 +245,11 @@ class QuantizedKVCache:
             raise ValueError("csaq-b200: out must have q's shape and dtype and rows of even stride")
         if workspace is None:
             workspace = self.workspace(S, Hq)
-        part, tickets = workspace.part, workspace.tickets
-        L = lib()
-        if part.device != self.device or tickets.device != self.device \
-                or part.numel() < L.csaq_kvq_attention_workspace_floats(self.batch, S, Hq, self.kv_heads, self.head_dim,
-                                                                        self.max_len) \
-                or tickets.numel() < L.csaq_kvq_attention_tickets(self.batch, S, Hq, self.kv_heads):
+        part = workspace.part
+        if part.device != self.device or part.numel() < self._floats(S, Hq):
             raise ValueError(f"csaq-b200: the workspace is too small for {S} tokens and {Hq} heads of this cache")
-        self._run(L.csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, pos0.data_ptr(),
+        self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, pos0.data_ptr(),
                   self.batch, S, Hq, self.kv_heads, self.head_dim,
                   float(scale) if scale is not None else 1.0 / math.sqrt(self.head_dim), part.data_ptr(),
-                  tickets.data_ptr(), out.data_ptr(), out.stride(0), dtype_code(q.dtype), stream_of(q))
+                  out.data_ptr(), out.stride(0), dtype_code(q.dtype), stream_of(q))
         return out

@@ -427,17 +427,16 @@ int csaq_kvq_read(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D
 /* csaq_decode_attention against a quantised cache: token (b, s), row b*S+s of q
  * (Hq*D wide, ldq elements apart), attends keys 0 .. min(pos0[b]+s, Lmax-1); a
  * token at a negative position sees nothing and its output is 0 (an unused
- * sequence of a batch: pos0[b] = -S). Any S. out rows are ldo elements apart.
- * part: csaq_kvq_attention_workspace_floats floats; tickets:
- * csaq_kvq_attention_tickets int32, zero before the first call (calls leave them
- * zero); calls that may overlap on the GPU need a workspace each. A token's
- * result does not depend on S or on the other sequences. */
+ * sequence of a batch: pos0[b] = -S). Any S. q needs 16-byte alignment and ldq a
+ * multiple of 8; out rows are ldo (even) elements apart. part:
+ * csaq_kvq_attention_workspace_floats floats of scratch (8-byte aligned, null when
+ * that is 0), rewritten by each call: calls that may overlap on the GPU need one
+ * each. A token's result does not depend on S or on the other sequences. */
 int64_t csaq_kvq_attention_workspace_floats(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t Lmax);
-int64_t csaq_kvq_attention_tickets(int64_t B, int64_t S, int64_t Hq, int64_t Hkv);
 int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cache* cache, const int32_t* pos0, int64_t B,
-                       int64_t S, int64_t Hq, int64_t Hkv, int64_t D, float scale, float* part, int32_t* tickets,
-                       void* out, int64_t ldo, int dtype, void* stream);
+                       int64_t S, int64_t Hq, int64_t Hkv, int64_t D, float scale, float* part, void* out,
+                       int64_t ldo, int dtype, void* stream);
 
 /* HF LlamaMLP gate: h = dtype(silu(g)) * u. */
 int csaq_silu_mul(const void* g, int64_t ldg, const void* u, int64_t ldu, void* h, int64_t ldh,

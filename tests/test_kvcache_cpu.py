@@ -30,7 +30,7 @@ def test_cache_descriptor_refused(bad, rc):
     c = _cache(**bad)
     assert L.csaq_kvq_write(None, 0, P, 1024, P, 1024, P, 1, 1, 0, 8, 128, None, None, 0, None, c, 2, None) == rc
     assert L.csaq_kvq_read(c, 1, 8, 128, 0, 1, P, P, 2, None) == rc
-    assert L.csaq_kvq_attention(P, 4096, c, P, 1, 1, 32, 8, 128, 0.1, P, P, P, 4096, 2, None) == rc
+    assert L.csaq_kvq_attention(P, 4096, c, P, 1, 1, 32, 8, 128, 0.1, P, P, 4096, 2, None) == rc
     assert L.csaq_kvq_read(None, 1, 8, 128, 0, 1, P, P, 2, None) == ARG
 
 
@@ -67,31 +67,29 @@ def test_attention_refusals():
     from csaq._lib import lib
     L = lib()
 
-    def call(q=P, ldq=4096, pos0=P, B=1, S=1, Hq=32, Hkv=8, D=128, part=P, tickets=P, out=P, ldo=4096, dtype=2):
-        return L.csaq_kvq_attention(q, ldq, _cache(), pos0, B, S, Hq, Hkv, D, 0.1, part, tickets, out, ldo, dtype, None)
+    def call(q=P, ldq=4096, pos0=P, B=1, S=1, Hq=32, Hkv=8, D=128, part=P, out=P, ldo=4096, dtype=2, Lmax=64):
+        return L.csaq_kvq_attention(q, ldq, _cache(Lmax=Lmax), pos0, B, S, Hq, Hkv, D, 0.1, part, out, ldo, dtype, None)
 
-    for bad in (dict(q=None), dict(pos0=None), dict(part=None), dict(tickets=None), dict(out=None), dict(S=0),
+    for bad in (dict(q=None), dict(pos0=None), dict(part=None, Lmax=1 << 20), dict(out=None), dict(S=0),
                 dict(Hq=0), dict(Hq=33), dict(ldq=4095), dict(ldo=4095), dict(dtype=0)):
         assert call(**bad) == ARG, bad
     for bad in (dict(ldo=4097), dict(out=ctypes.c_void_p(258)), dict(part=ctypes.c_void_p(260)), dict(S=70000),
-                dict(B=1 << 30)):
+                dict(B=1 << 30), dict(ldq=4098), dict(q=ctypes.c_void_p(264))):
         assert call(**bad) == UNSUPPORTED, bad
     assert L.csaq_kvq_attention_workspace_floats(1, 1, 33, 8, 128, 64) == -1
     assert L.csaq_kvq_attention_workspace_floats(1, 0, 32, 8, 128, 64) == -1
-    assert L.csaq_kvq_attention_tickets(0, 1, 32, 8) == -1
 
 
 def test_workspace_sizes():
-    """One partial state per (chunk, query row); the chunk grows with the cache so
-    that the pieces stay bounded, and does not depend on the step's tokens."""
+    """None while a head's chunks fit a cluster, else one partial state per (chunk,
+    query row): their number stays bounded and does not depend on the step's tokens."""
     from csaq._lib import lib
-    f, t = lib().csaq_kvq_attention_workspace_floats, lib().csaq_kvq_attention_tickets
-    assert f(1, 1, 32, 8, 128, 128) == 8 * 1 * 4 * 130
-    assert f(1, 5, 32, 8, 128, 640) == 5 * f(1, 1, 32, 8, 128, 640)
+    f = lib().csaq_kvq_attention_workspace_floats
+    assert f(1, 1, 32, 8, 128, 64) == 0 and f(128, 1, 32, 8, 128, 1 << 16) == 0
+    long = f(1, 1, 32, 8, 128, 1 << 17)
+    assert long > 0 and long % (8 * 4 * 130) == 0 and f(1, 5, 32, 8, 128, 1 << 17) == 5 * long
     for B, Hkv, Lmax in ((1, 8, 1 << 20), (64, 8, 1 << 15), (1, 1, 1 << 24), (2048, 16, 4096)):
-        pieces = f(B, 1, Hkv, Hkv, 64, Lmax) // 66
-        assert pieces <= max(B * Hkv, 4 * 2 * 148)
-    assert t(2, 5, 32, 8) == 2 * 8 * 3 and t(1, 1, 8, 8) == 8
+        assert f(B, 1, Hkv, Hkv, 64, Lmax) // 66 <= 4 * 148
 
 
 def test_struct_layout():

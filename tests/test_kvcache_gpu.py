@@ -345,7 +345,7 @@ def test_attention_independent_of_the_step(bits, D, group):
 
 def test_attention_strides_workspaces_and_repeats():
     """Padded rows of q and out (the padding stays), an own workspace used over and
-    over with other lengths and token counts, tickets left at zero, equal bits."""
+    over with other lengths and token counts, equal bits."""
     B, Hq, Hkv, D, L = 2, 8, 2, 128, 2000
     c = _filled(B, Hkv, L, D, 8, 64, seed=31)
     ws = c.workspace(4, Hq)
@@ -356,13 +356,15 @@ def test_attention_strides_workspaces_and_repeats():
         q = wide[:, :Hq * D]
         buf = torch.full((B * S, Hq * D + 6), 7.0, dtype=torch.bfloat16, device=DEV)
         out = c.attend(q, pos0, out=buf[:, :Hq * D], workspace=ws)
-        assert (buf[:, Hq * D:] == 7).all() and int(ws.tickets.abs().sum()) == 0
+        assert (buf[:, Hq * D:] == 7).all()
         assert torch.equal(out, c.attend(q.contiguous(), pos0))
         _check_attention(out, q.contiguous(), c, pos, S, D ** -0.5)
         odd = torch.empty(B * S * Hq * D + 3, dtype=torch.bfloat16, device=DEV)[3:].view(B * S, Hq * D).copy_(q)
         assert torch.equal(c.attend(odd, pos0), out)  # rows the kernel cannot read in place are copied
+    big = _cache(1, 2, 1 << 20, 128, 4, 64)  # chunks that meet in global memory
     with pytest.raises(ValueError, match="workspace"):
-        c.attend(torch.zeros(B * 5, Hq * D, dtype=torch.bfloat16, device=DEV), pos0, workspace=ws)
+        big.attend(torch.zeros(5, 1024, dtype=torch.bfloat16, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
+                   workspace=big.workspace(4, 8))
 
 
 def test_decode_loop_captured():
