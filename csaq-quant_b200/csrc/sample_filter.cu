@@ -15,11 +15,23 @@
 // the fp32 rate), and no sum goes through an atomic: every order is fixed.
 //
 // A cluster of CTAs takes one row and keeps it in shared memory as ordered integer
-// keys (one pass over the logits). A cut (of top-k over counts, of top-p over
-// masses) is found four key bits at a time: every thread adds its elements into 16
-// bins of its own, the bins are summed in a fixed order over threads and CTAs, and
-// the next pass looks only at the bin that holds the cut. The passes start at the
-// range of keys whose weight is not negligible.
+// keys: one pass over the logits. What follows depends on the row's settings:
+//
+//  list    top-k up to kListK: a histogram of counts over bins of 1/32 nat below the
+//          largest logit says which bins hold the first k ranks; their tokens, little
+//          more than k, are gathered in one CTA, sorted, cut and drawn from there.
+//  nucleus top-p alone: a histogram of (approximate) masses says near which bin the cut
+//          lies; the exact mass above three bins and the sorted tokens of the three
+//          give the cut, and a last pass over the row draws under it.
+//  digits  anything else that cuts, and what the two above hand over (more tokens than
+//          the list holds, a cut out of the bins' range): the cut is found three key
+//          bits at a time; every thread adds its elements into 8 bins of its own, the
+//          bins are summed in a fixed order over threads and CTAs, and the next pass
+//          looks only at the bin that holds the cut.
+//  none    no top-k, no top-p: the last pass alone.
+//
+// The histograms go through integer atomics and only say where to look; the answer
+// never depends on them.
 
 #include <atomic>
 
@@ -28,12 +40,16 @@
 namespace csaq {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kBins = 16;  // one warp sums one bin
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 8, kDigit = 3;  // of the digit passes; two warps sum a bin
+constexpr int kHist = 1024;           // bins of 1 / kPerNat below the largest logit
+constexpr float kPerNat = 32.0f;
+constexpr int kList = 2048;           // tokens that are sorted at most
+constexpr int kListK = 1024;          // ranks that a list may keep
 constexpr int kMaxCluster = 8;
 constexpr int kTable = 256;           // 2^(j / 256)
 constexpr double kNegligible = -50.0;  // exp below this is taken as 0: 2e-22 of the largest weight
-static_assert(kBins * 32 == kThreads, "a warp per bin");
+static_assert(kBins * 2 == kWarps && kList == 4 * kThreads && kHist == 2 * kThreads, "shares of a thread");
 
 struct FilterArgs {
   const void* logits;
@@ -104,18 +120,32 @@ __device__ __forceinline__ double remote_f64(const double* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ uint64_t remote_u64(const uint64_t* p, uint32_t rank) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t remote_u32(const uint32_t* p, uint32_t rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
 
-// exp(z) for z in [kNegligible, 0]: table-driven reduction (Tang 1989): z = n ln2 / 256 + r,
-// exp z = 2^(n / 256) (1 + r + .. + r^4 / 24), |r| <= 0.00136: within 4e-15 of it
-__device__ __forceinline__ double exp_tab(double z, const double* tab) {
-  const double t = rint(z * 369.3299304675746);  // 256 / ln 2
-  const int n = (int)t;
-  const double r = fma(t, -0.0027076061740622863, z);  // ln 2 / 256
+// a float's value as a double, by bits (subnormals come out near 2^-127, which next to
+// another logit is all the same)
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+
+// exp(d / T) for d / T in [kNegligible, 0], c = 256 / (T ln 2), it = 1 / T: table-driven
+// reduction (Tang 1989): d / T = n ln2 / 256 + r, exp = 2^(n / 256) (1 + r + .. + r^4 / 24),
+// |r| <= 0.00136: within 4e-15 of it
+__device__ __forceinline__ double exp_tab(double d, double c, double it, const double* tab) {
+  const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's low word is the rounded integer
+  const double t = fma(d, c, magic);
+  const int n = __double2loint(t);
+  const double r = fma(t - magic, -0.0027076061740622863, d * it);  // ln 2 / 256
   double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
   p = fma(r, p, 0.5);
   p = fma(r, p, 1.0);
@@ -124,19 +154,83 @@ __device__ __forceinline__ double exp_tab(double z, const double* tab) {
   return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
 }
 
-// What every CTA of the row knows; `red` is read by the other CTAs.
+// Static shared memory; what other CTAs read is marked.
 struct Shared {
   double tab[kTable];
-  double red[2][kBins];  // this CTA's bin sums, alternating from pass to pass
+  double red[2][kBins];  // read by others: this CTA's bin sums, alternating from pass to pass
   double tot[kBins];     // the row's
-  double scan[kThreads / 32];
-  uint32_t iscan[kThreads / 32];
-  double x_mass;  // exchanged at the end
-  uint32_t x_ties;
-  uint32_t x_max;
-  uint32_t wmax[kThreads / 32];
+  double half[kWarps];
+  double scan[kWarps];
+  uint32_t iscan[kWarps];
+  double x_mass;     // read by others
+  double x_above;    // read by others
+  uint32_t x_ties;   // read by others
+  uint32_t x_max;    // read by others
+  uint32_t x_count;  // read by others: tokens in this CTA's list
+  uint32_t x_key, x_keep;  // read by others (CTA 0): the cut of a nucleus; x_keep 0: none was found
+  uint32_t wmax[kWarps];
   int pick;
+  uint32_t at;
+  uint32_t hist[kHist];  // read by others
 };
+
+// exclusive prefix sums of N doubles a thread in thread order; the total
+template <int N>
+__device__ __forceinline__ double block_scan(const double (&v)[N], double (&before)[N], double* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mine += v[i];
+  double incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  double wb = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) wb += warp_sums[w];
+    all += warp_sums[w];
+  }
+  double x = __shfl_up_sync(0xffffffffu, incl, 1);
+  x = wb + (lane == 0 ? 0.0 : x);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    before[i] = x;
+    x += v[i];
+  }
+  return all;
+}
+__device__ __forceinline__ double block_sum(double v, double* warp_sums) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) all += warp_sums[w];
+  return all;
+}
+
+// bitonic sort of n (a power of two, at most kList) in shared memory, largest first
+__device__ __forceinline__ void sort_down(uint64_t* v, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const uint64_t x = v[a], y = v[b];
+        if ((x < y) == ((a & size) == 0)) v[a] = y, v[b] = x;
+      }
+    }
+  __syncthreads();
+}
+__device__ __forceinline__ int pow2_from(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
 template <typename T>
 struct Row {
@@ -144,18 +238,36 @@ struct Row {
   using K = typename KO::K;
   const K* keys;  // the slice, in index order
   int n;
+  int64_t first;  // index of its first element
   Shared* sh;
-  double* hist;  // [bin][thread]
+  uint8_t* work;  // kWorkBytes: the bins of the digit passes, or the list
   uint32_t rank, nc;
   int parity;
   bool top_inf;  // the largest logit is +inf: its like have weight 1, all else 0
-  double xmax, inv_t;
+  double xmax, inv_t, scale_t, lowest;
+  float fmax, per_bin;
   uint32_t kmax;
 
   __device__ __forceinline__ double weight(uint32_t k) const {
     if (top_inf) return k == kmax ? 1.0 : 0.0;
-    const double z = ((double)KO::value(k) - xmax) * inv_t;
-    return z >= kNegligible ? exp_tab(z, sh->tab) : 0.0;
+    const double d = widen(KO::value(k)) - xmax;
+    return d >= lowest ? exp_tab(d, scale_t, inv_t, sh->tab) : 0.0;
+  }
+  // bins below the largest logit, in exact order of the keys; kHist and more: none
+  __device__ __forceinline__ float depth(uint32_t k) const { return (fmax - KO::value(k)) * per_bin; }
+
+  // f(key) over the slice, and f(key, position)
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    constexpr int PER = 16 / (int)sizeof(K);
+    const int whole = n / PER;
+    for (int i = threadIdx.x; i < whole; i += kThreads) {
+      const uint4 u = reinterpret_cast<const uint4*>(keys)[i];
+      const K* e = reinterpret_cast<const K*>(&u);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) f((uint32_t)e[j], i * PER + j);
+    }
+    for (int i = whole * PER + threadIdx.x; i < n; i += kThreads) f((uint32_t)keys[i], i);
   }
 
   struct Cut {
@@ -170,34 +282,38 @@ struct Row {
   // when 0). COUNT: weights 1 and target `bound`; else masses and target bound * total.
   template <bool COUNT>
   __device__ Cut select(uint32_t klo, double bound, uint32_t alone, double alone_w) {
+    double* hist = reinterpret_cast<double*>(work);  // [bin][thread]
     const uint32_t span = kmax - klo;
     const int bits = 32 - __clz(span | 1u);
     uint32_t prefix = 0;
     Cut c{klo, 0.0, 0.0, bound};
-    bool first = true;
-    for (int shift = (bits - 1) / 4 * 4; shift >= 0; shift -= 4) {
+    bool first_pass = true;
+    __syncthreads();
+    for (int shift = (bits - 1) / kDigit * kDigit; shift >= 0; shift -= kDigit) {
 #pragma unroll
       for (int b = 0; b < kBins; ++b) hist[b * kThreads + threadIdx.x] = 0.0;
-      auto add = [&](uint32_t k) {
+      each([&](uint32_t k, int) {
         const uint32_t o = k - klo;  // keys below klo wrap around to far above the span
-        if (o > span || k == alone || (!first && (o >> (shift + 4)) != prefix)) return;
-        double* h = &hist[((o >> shift) & 15u) * kThreads + threadIdx.x];
-        *h += COUNT ? 1.0 : weight(k);
-      };
-      for (int i = threadIdx.x; i < n; i += kThreads) add(keys[i]);
+        if (o > span || k == alone || (!first_pass && (o >> (shift + kDigit)) != prefix)) return;
+        hist[((o >> shift) & (kBins - 1)) * kThreads + threadIdx.x] += COUNT ? 1.0 : weight(k);
+      });
       if (alone_w != 0.0 && rank == 0 && threadIdx.x == 0) {
         const uint32_t o = alone - klo;
-        if (o <= span && (first || (o >> (shift + 4)) == prefix)) hist[((o >> shift) & 15u) * kThreads] += alone_w;
+        if (o <= span && (first_pass || (o >> (shift + kDigit)) == prefix))
+          hist[((o >> shift) & (kBins - 1)) * kThreads] += alone_w;
       }
       __syncthreads();
       {
-        const int b = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int w = threadIdx.x >> 5, b = w >> 1, lane = threadIdx.x & 31;
         double s = 0.0;
-        for (int i = lane; i < kThreads; i += 32) s += hist[b * kThreads + i];
+#pragma unroll
+        for (int i = 0; i < kThreads / 64; ++i) s += hist[b * kThreads + (w & 1) * (kThreads / 2) + i * 32 + lane];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sh->red[parity][b] = s;
+        if (lane == 0) sh->half[w] = s;
       }
+      __syncthreads();
+      if (threadIdx.x < kBins) sh->red[parity][threadIdx.x] = sh->half[2 * threadIdx.x] + sh->half[2 * threadIdx.x + 1];
       cluster_sync();
       if (threadIdx.x < kBins) {
         double s = 0.0;
@@ -206,7 +322,7 @@ struct Row {
       }
       __syncthreads();
       parity ^= 1;
-      if (first && !COUNT) {
+      if (first_pass && !COUNT) {
         double z = 0.0;
         for (int b = kBins - 1; b >= 0; --b) z += sh->tot[b];
         c.target = bound * z;
@@ -218,14 +334,73 @@ struct Row {
         if (s > 0.0 && above <= c.target) pick = b, c.base = above, c.mass = s;
         above += s;
       }
-      prefix = (prefix << 4) | (uint32_t)pick;
-      first = false;
+      prefix = (prefix << kDigit) | (uint32_t)pick;
+      first_pass = false;
       __syncthreads();  // tot is rewritten by the next pass
     }
     c.key = klo + prefix;
     return c;
   }
+
+  // This CTA's histogram: counts, or masses as 2^15 w / 2^-bin (bin in units of 1 /
+  // kPerNat nat); for masses the exact sum of the slice's weights comes back.
+  template <bool COUNT>
+  __device__ double histogram() {
+    for (int i = threadIdx.x; i < kHist; i += kThreads) sh->hist[i] = 0;
+    __syncthreads();
+    double z = 0.0;
+    each([&](uint32_t k, int) {
+      if (k == 0) return;
+      const float u = depth(k);
+      if (!COUNT) z += weight(k);
+      if (u < (float)kHist) {
+        const int b = (int)u;
+        atomicAdd(&sh->hist[b], COUNT ? 1u : (uint32_t)(32768.0f * __expf(((float)b - u) * (1.0f / kPerNat))));
+      }
+    });
+    return COUNT ? 0.0 : block_sum(z, sh->scan);
+  }
+  // The row's histogram, bins 2 t and 2 t + 1 of thread t (after a cluster_sync).
+  __device__ __forceinline__ void row_bins(double (&v)[2]) const {
+    v[0] = v[1] = 0.0;
+    for (uint32_t r = 0; r < nc; ++r) {
+      v[0] += (double)remote_u32(&sh->hist[2 * threadIdx.x], r);
+      v[1] += (double)remote_u32(&sh->hist[2 * threadIdx.x + 1], r);
+    }
+  }
+  // The elements with lo <= depth < hi into this CTA's list; sh->x_count of them, or more than it holds.
+  __device__ void gather(float lo, float hi) {
+    uint64_t* list = reinterpret_cast<uint64_t*>(work);
+    if (threadIdx.x == 0) sh->x_count = 0;
+    __syncthreads();
+    each([&](uint32_t k, int i) {
+      if (k == 0) return;
+      const float u = depth(k);
+      if (u >= lo && u < hi) {
+        const uint32_t at = atomicAdd(&sh->x_count, 1u);
+        if (at < (uint32_t)kList) list[at] = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)(first + i));
+      }
+    });
+  }
+  // CTA 0: all lists, sorted by rank (after a cluster_sync); the others are done with
+  // theirs at the next one. -1: too many.
+  __device__ int collect() {
+    uint64_t* list = reinterpret_cast<uint64_t*>(work);
+    uint32_t total = sh->x_count;
+    for (uint32_t r = 1; r < nc; ++r) {
+      const uint32_t c = remote_u32(&sh->x_count, r);
+      if (total + c <= (uint32_t)kList)
+        for (uint32_t i = threadIdx.x; i < c; i += kThreads) list[total + i] = remote_u64(list + i, r);
+      total += c;
+    }
+    if (total > (uint32_t)kList) return -1;
+    const int size = pow2_from((int)total);
+    for (int i = (int)total + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    sort_down(list, size);
+    return (int)total;
+  }
 };
+constexpr int kWorkBytes = kBins * kThreads * 8 > kList * 8 * 2 ? kBins * kThreads * 8 : kList * 8 * 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArgs a) {
@@ -238,8 +413,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   const uint32_t rank = cluster_rank(), nc = cluster_size();
   const int64_t m = blockIdx.x / nc;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  double* hist = reinterpret_cast<double*>(dyn);
-  K* keys = reinterpret_cast<K*>(dyn + kBins * kThreads * sizeof(double));
+  K* keys = reinterpret_cast<K*>(dyn + kWorkBytes);
   const int64_t lo = (int64_t)rank * a.chunk;
   const int n = (int)(lo >= a.V ? 0 : (a.V - lo < a.chunk ? a.V - lo : a.chunk));
   if (tid < kTable) sh.tab[tid] = exp2((double)tid / kTable);
@@ -304,12 +478,16 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   if (u >= 1.0) u = 1.0 - 0x1p-53;
 
   Row<T> row;
-  row.keys = keys, row.n = n, row.sh = &sh, row.hist = hist, row.rank = rank, row.nc = nc, row.parity = 0;
+  row.keys = keys, row.n = n, row.first = lo, row.sh = &sh, row.work = dyn, row.rank = rank, row.nc = nc, row.parity = 0;
   row.kmax = kmax;
   const float xmax = KO::value(kmax);
   row.top_inf = xmax == INFINITY;
-  row.xmax = xmax;
+  row.xmax = widen(xmax);
   row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
+  row.scale_t = row.inv_t * (kTable / 0.6931471805599453);
+  row.lowest = kNegligible / row.inv_t;
+  row.fmax = xmax;
+  row.per_bin = fminf((float)(row.inv_t * kPerNat), 1e30f);
 
   // the lowest key that can have weight: a little below max + kNegligible T
   uint32_t klo = kmax;
@@ -319,25 +497,165 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     if (klo == 0 || klo > kmax) klo = 1u;
   }
 
-  // the cut: keys above ckey are kept, and the first ckeep of those at it
+  const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0f && !greedy;  // a NaN top_p switches it off
+  const double p = top_p > 0.0f ? (double)top_p : 0.0;
+  // keys above ckey are kept, and the first cties of those at it
   uint32_t ckey = klo, cties = 0xffffffffu;
-  uint32_t alone = 0;
-  double alone_w = 0.0;
-  if (top_k > 0 && top_k < a.V) {
-    const auto c = row.template select<true>(klo, (double)(top_k - 1), 0u, 0.0);
-    ckey = c.key;
-    const double keep = (double)top_k - c.base;  // of c.mass ties
-    cties = (uint32_t)(keep < c.mass ? keep : c.mass);
-    alone = ckey;
-    alone_w = (double)cties * row.weight(ckey);
+  bool digits = cut_k || cut_p;
+  // where differences of logits and their bins cannot overflow into one another
+  const bool binned = fabsf(xmax) <= 1e38f && (greedy || temp <= 1e30f);
+
+  if (cut_k && top_k <= kListK && binned) {
+    row.template histogram<true>();
+    cluster_sync();
+    double v[2], before[2];
+    row.row_bins(v);
+    if (tid == 0) sh.at = kHist;
+    block_scan<2>(v, before, sh.scan);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // the bin that the k-th rank falls into
+      if (before[i] < (double)top_k && before[i] + v[i] >= (double)top_k) sh.at = 2 * tid + i;
+    __syncthreads();
+    const uint32_t at = sh.at;
+    if (at < kHist) {
+      row.gather(0.0f, (float)(at + 1));
+      cluster_sync();
+      uint32_t total = 0;
+      for (uint32_t r = 0; r < nc; ++r) total += remote_u32(&sh.x_count, r);
+      if (total <= (uint32_t)kList) {
+        if (rank == 0) {
+          uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
+          const int m1 = min(row.collect(), top_k);  // ranks 0 .. m1 - 1 pass top-k
+          double w[2], above[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < m1 ? row.weight((uint32_t)(list[2 * tid + i] >> 32)) : 0.0;
+          const double z = block_scan<2>(w, above, sh.scan);
+          double* by_rank = reinterpret_cast<double*>(dyn) + kList;
+          if (tid == 0) sh.at = 0;
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = 2 * tid + i;
+            if (r >= m1) continue;
+            by_rank[r] = w[i];
+            // both cuts keep a first part of the ranks, the first rank always
+            if (r == 0 || ((!cut_p || above[i] <= p * z) && w[i] >= min_p)) atomicMax(&sh.at, (uint32_t)r + 1u);
+          }
+          __syncthreads();
+          const int kept = (int)sh.at, size = pow2_from(kept);
+          uint64_t mine[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = 2 * tid + i;
+            mine[i] = r < kept ? (list[r] << 32 | (uint32_t)r) : 0;  // the low half rises as the index falls
+          }
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (2 * tid + i < size) list[2 * tid + i] = mine[i];
+          sort_down(list, size);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < kept ? by_rank[(uint32_t)list[2 * tid + i]] : 0.0;
+          const double mass = block_scan<2>(w, above, sh.scan);
+          const double target = u * mass;
+          if (tid == 0) sh.pick = kept - 1;  // when rounding lets none pass
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (2 * tid + i < kept && above[i] + w[i] > target) atomicMin(&sh.pick, 2 * tid + i);
+          __syncthreads();
+          if (tid == 0) a.out[m] = (int64_t)(0xffffffffu - (uint32_t)(list[sh.pick] >> 32));
+        }
+        cluster_sync();  // no CTA leaves while another reads its shared memory
+        return;
+      }
+    }
+  } else if (cut_p && !cut_k && binned) {
+    const double zc = row.template histogram<false>();
+    if (tid == 0) sh.x_mass = zc, sh.at = kHist;
+    cluster_sync();
+    double z = 0.0;
+    for (uint32_t r = 0; r < nc; ++r) z += remote_f64(&sh.x_mass, r);
+    const double target = p * z;
+    double v[2], before[2];
+    row.row_bins(v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] *= 0x1p-15 * exp_tab(-(double)(2 * tid + i), kTable / 0.6931471805599453 / kPerNat, 1.0 / kPerNat, sh.tab);
+    block_scan<2>(v, before, sh.scan);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (before[i] <= target && before[i] + v[i] > target) atomicMin(&sh.at, 2u * tid + i);
+    __syncthreads();
+    const uint32_t at = sh.at;
+    if (at < kHist) {
+      const float w0 = at > 0 ? (float)(at - 1) : 0.0f, w1 = (float)(at + 2);
+      row.gather(w0, w1);
+      double above = 0.0;
+      row.each([&](uint32_t k, int) {
+        if (k != 0 && row.depth(k) < w0) above += row.weight(k);
+      });
+      above = block_sum(above, sh.scan);
+      if (tid == 0) sh.x_above = above;
+      cluster_sync();
+      if (rank == 0) {
+        uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
+        const int total = row.collect();
+        if (tid == 0) sh.x_keep = 0, sh.at = 0;
+        if (total > 0) {
+          double base = 0.0;
+          for (uint32_t r = 0; r < nc; ++r) base += remote_f64(&sh.x_above, r);
+          double w[4], before4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = 4 * tid + i < total ? row.weight((uint32_t)(list[4 * tid + i] >> 32)) : 0.0;
+          const double inside = block_scan<4>(w, before4, sh.scan);
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * tid + i < total && base + before4[i] <= target) atomicMax(&sh.at, 4u * tid + i + 1u);
+          __syncthreads();
+          const uint32_t kept = sh.at;  // of the list; the cut lies inside it when its ends say so
+          if (kept > 0 && base + inside > target) {
+            const uint32_t key = (uint32_t)(list[kept - 1] >> 32);
+            uint32_t same = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              same += 4u * tid + i < kept && (uint32_t)(list[4 * tid + i] >> 32) == key ? 1u : 0u;
+            same = __reduce_add_sync(0xffffffffu, same);
+            if (lane == 0 && same) atomicAdd(&sh.x_keep, same);
+            if (tid == 0) sh.x_key = key;
+          }
+        }
+      }
+      cluster_sync();
+      const uint32_t keep = remote_u32(&sh.x_keep, 0);
+      if (keep > 0) {
+        ckey = remote_u32(&sh.x_key, 0);
+        cties = keep;
+        digits = false;
+      }
+    }
   }
-  if (top_p < 1.0f && !greedy) {  // NaN switches it off
-    const auto c = row.template select<false>(ckey, top_p > 0.0f ? (double)top_p : 0.0, alone, alone_w);
-    const double w = row.weight(c.key);
-    const uint32_t all = (uint32_t)rint(c.mass / w);
-    const double more = floor((c.target - c.base) / w);
-    ckey = c.key;
-    cties = more + 1.0 < (double)all ? (uint32_t)more + 1u : all;
+  if (digits) {
+    uint32_t alone = 0;
+    double alone_w = 0.0;
+    if (cut_k) {
+      const auto c = row.template select<true>(klo, (double)(top_k - 1), 0u, 0.0);
+      ckey = c.key;
+      const double keep = (double)top_k - c.base;  // of c.mass ties
+      cties = (uint32_t)(keep < c.mass ? keep : c.mass);
+      alone = ckey;
+      alone_w = (double)cties * row.weight(ckey);
+    }
+    if (cut_p) {
+      const auto c = row.template select<false>(ckey, p, alone, alone_w);
+      const double w = row.weight(c.key);
+      const uint32_t all = (uint32_t)rint(c.mass / w);
+      const double more = floor((c.target - c.base) / w);
+      ckey = c.key;
+      cties = more + 1.0 < (double)all ? (uint32_t)more + 1u : all;
+    }
   }
 
   // kept weight above the cut and ties at it, per contiguous segment of a thread
@@ -375,7 +693,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   if (tid == 0) {
     double s = 0.0;
     uint32_t t = 0;
-    for (int w = 0; w < kThreads / 32; ++w) s += sh.scan[w], t += sh.iscan[w];
+    for (int w = 0; w < kWarps; ++w) s += sh.scan[w], t += sh.iscan[w];
     sh.x_mass = s;
     sh.x_ties = t;
   }
@@ -450,16 +768,16 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-constexpr int kHistBytes = kBins * kThreads * 8;
 constexpr int kSmemMax = 200 * 1024;  // dynamic, beside the static struct
 
 template <typename T>
 int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
-  constexpr int per = (kSmemMax - kHistBytes) / (int)sizeof(typename KeyOf<T>::K) / 8 * 8;
-  // CTAs of a row: as many as its keys need, and up to 8 while the rows alone
-  // leave SMs idle
+  constexpr int per = (kSmemMax - kWorkBytes) / (int)sizeof(typename KeyOf<T>::K) / 8 * 8;
+  // CTAs of a row: as many as leave two places an SM (by shared memory), and up to 8
+  // while the rows alone leave SMs idle
+  constexpr int two = (110 * 1024 - kWorkBytes - (int)sizeof(Shared)) / (int)sizeof(typename KeyOf<T>::K);
   int nc = 1;
-  while (nc < kMaxCluster && ((a.V + nc - 1) / nc > per - 8 || rows * nc * 2 <= 148)) nc *= 2;
+  while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * nc <= 148)) nc *= 2;
   const int64_t chunk = ((a.V + nc - 1) / nc + 7) / 8 * 8;
   if (chunk > per) return CSAQ_ERR_UNSUPPORTED;
   a.chunk = (int)chunk;
@@ -477,7 +795,7 @@ int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * nc));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kHistBytes + chunk * sizeof(typename KeyOf<T>::K);
+    cfg.dynamicSmemBytes = kWorkBytes + chunk * sizeof(typename KeyOf<T>::K);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -484,7 +484,7 @@ typedef struct csaq_sample_params {
  * times the kept mass. Weights and sums are fp64 and their order is fixed. NaN
  * and -inf logits are never drawn, +inf ones share the whole mass; a row of NaN
  * and -inf gives -1. Rows are n_parts slices like csaq_sample_rows; a row of
- * up to 270,000 fp32 or 550,000 16-bit logits (else CSAQ_ERR_UNSUPPORTED). */
+ * up to 340,000 fp32 or 680,000 16-bit logits (else CSAQ_ERR_UNSUPPORTED). */
 int csaq_sample_filtered(const void* logits, int n_parts, int64_t part_stride, int64_t ld, int64_t part_len,
                          int64_t rows, const csaq_sample_params* params, const float* random, int64_t* out, int dtype,
                          void* stream);

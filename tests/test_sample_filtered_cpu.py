@@ -21,7 +21,7 @@ def test_c_refusals():
                  (P, 2, -8, 8, 8, 1, s, P, P, 0)):
         assert f(*args, None) == -1, args
     assert f(P, 1, 0, 8, 8, 0, s, P, P, 0, None) == 0  # no rows
-    for V, dtype in ((300_000, 0), (600_000, 1), (1 << 31, 2)):  # rows that no cluster holds
+    for V, dtype in ((400_000, 0), (700_000, 1), (1 << 31, 2)):  # rows that no cluster holds
         assert f(P, 1, 0, V, V, 1, s, P, P, dtype, None) == -5
 
 

@@ -37,7 +37,9 @@ SETTINGS = [dict(), dict(temperature=0.6), dict(top_k=1), dict(top_k=7, temperat
             dict(top_p=0.9), dict(top_p=0.3, temperature=0.8), dict(top_p=0.999), dict(min_p=0.05), dict(min_p=1.0),
             dict(top_k=50, top_p=0.95, min_p=0.02, temperature=0.8), dict(top_k=3, top_p=0.5, temperature=5.0),
             dict(top_k=20000, top_p=0.97, temperature=2.0), dict(temperature=0.0), dict(temperature=1e-3, top_p=0.9),
-            dict(temperature=100.0, top_k=300, top_p=0.7), dict(top_p=1e-9)]
+            dict(temperature=100.0, top_k=300, top_p=0.7), dict(top_p=1e-9), dict(top_k=1024, top_p=0.6),
+            dict(top_k=1025, min_p=0.001), dict(temperature=50.0, top_p=0.5), dict(temperature=1e-4, top_k=200),
+            dict(temperature=0.02, top_p=0.9999999), dict(temperature=1e31, top_k=9), dict(top_k=100, min_p=0.3)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -58,7 +60,7 @@ def test_small_and_odd_vocabularies(dtype, V):
         _check(x, u, sample_tokens(x.to(DEV), u.to(DEV), **kw), **kw)
 
 
-@pytest.mark.parametrize("rows,V,dtype", [(3, 550000, torch.bfloat16), (3, 270000, torch.float32), (160, 151936,
+@pytest.mark.parametrize("rows,V,dtype", [(3, 680000, torch.bfloat16), (3, 340000, torch.float32), (160, 151936,
                                           torch.bfloat16), (300, 32003, torch.float16), (200, 70000, torch.float32)])
 def test_large(rows, V, dtype):
     """The widest rows, and more rows than SMs: every cluster size."""
@@ -163,6 +165,28 @@ def test_flat_rows_hit_every_border_right(dtype, V):
     assert torch.equal(got, torch.floor(u.double() * V).long())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_crowded_cuts(dtype):
+    """More equal or nearly equal tokens at a cut than a list holds, in one and in many
+    CTAs, and cuts on either side of the crowd."""
+    from csaq.sampling import sample_tokens
+    V = 30000
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(6, V, generator=g) * 0.01
+    x[0] = 0.0                                    # all equal
+    x[1, ::3] = 1.0                               # 10000 equal leaders
+    x[2, 100:900] = 4.0                           # 800 leaders in one CTA, a dense crowd below
+    x[3] = torch.arange(V) * 1e-5                 # rising, finely
+    x[4, :2500] = 0.5
+    x[4, 2500:] = torch.randn(V - 2500, generator=g) - 3
+    x = x.to(dtype)
+    for seed, kw in enumerate((dict(top_k=500), dict(top_k=1000), dict(top_k=900), dict(top_p=0.5), dict(top_p=0.2),
+                               dict(top_p=0.95), dict(top_k=20000, top_p=0.4), dict(top_k=1000, top_p=0.999),
+                               dict(top_k=801, top_p=0.9999))):
+        u = torch.rand(6, generator=torch.Generator().manual_seed(seed))
+        _check(x, u, sample_tokens(x.to(DEV), u.to(DEV), **kw), **kw)
+
+
 def test_random_numbers_outside():
     """Below 0 and NaN count as 0, 1 and more as the largest number below 1."""
     from csaq.sampling import sample_tokens
@@ -236,4 +260,4 @@ def test_refusals_on_the_device():
             sample_tokens(*args, **kw)
     assert sample_tokens(x[:0], u[:0]).shape == (0,)
     with pytest.raises(RuntimeError, match="not supported"):
-        sample_tokens(torch.zeros(1, 600000, dtype=torch.bfloat16, device=DEV), u[:1])
+        sample_tokens(torch.zeros(1, 800000, dtype=torch.bfloat16, device=DEV), u[:1])
