@@ -11,8 +11,9 @@
 //
 // The answer is an index, so there is no tolerance to hide in: a vocabulary of
 // 128k has borders everywhere in [0, 1), and weights or sums in 32 bits would move
-// some of them across u. Weights and sums are therefore fp64 (B200 runs it at half
-// the fp32 rate), and no sum goes through an atomic: every order is fixed.
+// some of them across u. Sums are therefore fp64, weights good to 2^-32 and a function
+// of the key alone (their errors, one per value and of either sign, move a border by
+// some 1e-11), and no sum goes through an atomic: every order is fixed.
 //
 // A cluster of CTAs takes one row and keeps it in shared memory as ordered integer
 // keys: one pass over the logits. What follows depends on the row's settings:
@@ -34,6 +35,7 @@
 // never depends on them.
 
 #include <atomic>
+#include <cfloat>
 
 #include "common.cuh"
 
@@ -61,39 +63,55 @@ struct FilterArgs {
   int chunk;  // elements of a CTA's slice
 };
 
-// Keys order like the logits; 0 stands for NaN and -inf. -0 and +0 are one value.
+// Keys order like the logits, -0 and +0 as one value. kLow is -inf's: a key up to it is
+// -inf or a negative NaN's, one above kInf a positive NaN's (those are set to 0 before
+// use). keys(w): of the packed logits of a 32-bit word.
 template <typename T> struct KeyOf;
 template <> struct KeyOf<float> {
   using K = uint32_t;
-  static __device__ __forceinline__ K key(float x) {
-    if (x != x || x == -INFINITY) return 0u;
-    const uint32_t b = __float_as_uint(x + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+  static constexpr uint32_t kLow = 0x007fffffu, kInf = 0xff800000u;
+  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
+    const int b = __float_as_int(__uint_as_float(w) + 0.0f);
+    return (uint32_t)b ^ ((uint32_t)(b >> 31) | 0x80000000u);
   }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
   }
+  static __device__ __forceinline__ uint32_t max_in(uint32_t k) { return k; }  // of the keys of a word
+  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return max(a, b); }
 };
-template <typename T>
-struct KeyOf16 {
+struct Key16 {
   using K = uint16_t;
-  static __device__ __forceinline__ K key(T v) {
-    const float x = to_f32<T>(v);
-    if (x != x || x == -INFINITY) return 0;
-    const uint32_t b = x == 0.0f ? 0u : bits_of<T>(v);
-    return (K)(b & 0x8000u ? ~b : b | 0x8000u);
+  static __device__ __forceinline__ uint32_t ordered(uint32_t w) {
+    return w ^ (((w >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u);
   }
+  static __device__ __forceinline__ uint32_t max_in(uint32_t k) { return max(k & 0xffffu, k >> 16); }
+  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 };
-template <> struct KeyOf<__half> : KeyOf16<__half> {
+template <> struct KeyOf<__half> : Key16 {
+  static constexpr uint32_t kLow = 0x03ffu, kInf = 0xfc00u;
+  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
+    const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.0f));
+    return ordered(*reinterpret_cast<const uint32_t*>(&r));
+  }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __half2float(__ushort_as_half((unsigned short)(k & 0x8000u ? k & 0x7fffu : ~k)));
   }
 };
-template <> struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16> {
+template <> struct KeyOf<__nv_bfloat16> : Key16 {
+  static constexpr uint32_t kLow = 0x007fu, kInf = 0xff80u;
+  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
+    const __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.0f));
+    return ordered(*reinterpret_cast<const uint32_t*>(&r));
+  }
   static __device__ __forceinline__ float value(uint32_t k) {
-    return __bfloat162float(__ushort_as_bfloat16((unsigned short)(k & 0x8000u ? k & 0x7fffu : ~k)));
+    return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu) << 16);
   }
 };
+template <typename T>
+__device__ __forceinline__ typename KeyOf<T>::K key_of(T v) {
+  return (typename KeyOf<T>::K)KeyOf<T>::keys(bits_of<T>(v));
+}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -138,20 +156,23 @@ __device__ __forceinline__ double widen(float x) {
   return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 
-// exp(d / T) for d / T in [kNegligible, 0], c = 256 / (T ln 2), it = 1 / T: table-driven
-// reduction (Tang 1989): d / T = n ln2 / 256 + r, exp = 2^(n / 256) (1 + r + .. + r^4 / 24),
-// |r| <= 0.00136: within 4e-15 of it
-__device__ __forceinline__ double exp_tab(double d, double c, double it, const double* tab) {
-  const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's low word is the rounded integer
-  const double t = fma(d, c, magic);
-  const int n = __double2loint(t);
-  const double r = fma(t - magic, -0.0027076061740622863, d * it);  // ln 2 / 256
-  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-  p = fma(r, p, 0.5);
-  p = fma(r, p, 1.0);
-  p = fma(r, p, 1.0);
-  p *= tab[n & (kTable - 1)];
-  return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+// exp((v - x) / T) for a result of at least exp(kNegligible), with ch + cl = 256 / (T ln 2):
+// table-driven reduction (Tang 1989) in pairs of fp32. (v - x) exactly as d + e, its
+// product with ch + cl as n + f with n whole; exp = 2^(n / 256) (1 + r + r^2 / 2 + r^3 / 6),
+// r = f ln 2 / 256, |r| <= 0.00136. r is good to 2^-34 and so is the bracket; fp64 takes only
+// the last step (measured here at 12000 clocks for 16000 weights a CTA when it took all).
+__device__ __forceinline__ double exp_tab(float v, float x, float ch, float cl, const double* tab) {
+  const float d = v - x, dv = d - v, e = (v - (d - dv)) - (x + dv);
+  const float zh = d * ch;
+  const float zl = fmaf(e, ch, fmaf(d, cl, fmaf(d, ch, -zh)));
+  const float magic = 12582912.0f;  // 1.5 2^23: the sum's low bits are the rounded integer
+  const float t = zh + magic;
+  const int n = __float_as_int(t) - __float_as_int(magic);
+  const float r = ((zh - (t - magic)) + zl) * 0.0027076061740622863f;
+  const float q = fmaf(r * r, fmaf(r, 1.0f / 6.0f, 0.5f), r);
+  const double c = tab[n & (kTable - 1)];
+  const double w = fma(c, widen(q), c);
+  return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
 }
 
 // Static shared memory; what other CTAs read is marked.
@@ -166,12 +187,13 @@ struct Shared {
   double x_above;    // read by others
   uint32_t x_ties;   // read by others
   uint32_t x_max;    // read by others
+  uint32_t x_min, x_top;  // read by others: smallest and largest key of a window, or the first index
   uint32_t x_count;  // read by others: tokens in this CTA's list
   uint32_t x_key, x_keep;  // read by others (CTA 0): the cut of a nucleus; x_keep 0: none was found
   uint32_t wmax[kWarps];
   int pick;
   uint32_t at;
-  uint32_t hist[kHist];  // read by others
+  __align__(8) uint32_t hist[kHist];  // read by others
 };
 
 // exclusive prefix sums of N doubles a thread in thread order; the total
@@ -243,31 +265,42 @@ struct Row {
   uint8_t* work;  // kWorkBytes: the bins of the digit passes, or the list
   uint32_t rank, nc;
   int parity;
-  bool top_inf;  // the largest logit is +inf: its like have weight 1, all else 0
-  double xmax, inv_t, scale_t, lowest;
-  float fmax, per_bin;
+  float fmax, ch, cl, lowest, per_bin;  // largest logit, 256 / (T ln 2), the lowest logit with weight, bins
   uint32_t kmax;
 
+  // (no branch: the weights of a piece are computed side by side)
   __device__ __forceinline__ double weight(uint32_t k) const {
-    if (top_inf) return k == kmax ? 1.0 : 0.0;
-    const double d = widen(KO::value(k)) - xmax;
-    return d >= lowest ? exp_tab(d, scale_t, inv_t, sh->tab) : 0.0;
+    const float v = KO::value(k);
+    const double w = exp_tab(v, fmax, ch, cl, sh->tab);
+    return v >= lowest ? w : 0.0;
   }
   // bins below the largest logit, in exact order of the keys; kHist and more: none
   __device__ __forceinline__ float depth(uint32_t k) const { return (fmax - KO::value(k)) * per_bin; }
 
-  // f(key) over the slice, and f(key, position)
+  static constexpr int PER = 16 / (int)sizeof(K);  // keys of a 16-byte piece
+  // f(keys, position, count) over 16-byte pieces (the last one may hold fewer keys);
+  // pieces without a key from `from` on are passed over
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    constexpr int PER = 16 / (int)sizeof(K);
-    const int whole = n / PER;
-    for (int i = threadIdx.x; i < whole; i += kThreads) {
-      const uint4 u = reinterpret_cast<const uint4*>(keys)[i];
+  __device__ __forceinline__ void pieces(uint32_t from, F f) const {
+    for (int i = threadIdx.x * PER; i < n; i += kThreads * PER) {
+      const uint4 u = *reinterpret_cast<const uint4*>(keys + i);  // the buffer ends with a whole piece
+      const int count = min(PER, n - i);
+      if (KO::max_in(KO::max_of(KO::max_of(u.x, u.y), KO::max_of(u.z, u.w))) < from && count == PER) continue;
       const K* e = reinterpret_cast<const K*>(&u);
+      uint32_t k[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) f((uint32_t)e[j], i * PER + j);
+      for (int j = 0; j < PER; ++j) k[j] = j < count ? (uint32_t)e[j] : 0u;
+      f(k, i);
     }
-    for (int i = whole * PER + threadIdx.x; i < n; i += kThreads) f((uint32_t)keys[i], i);
+  }
+  // f(key, position) over the keys from `from` (at least 1) on
+  template <typename F>
+  __device__ __forceinline__ void each(uint32_t from, F f) const {
+    pieces(from, [&](const uint32_t (&k)[PER], int i) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (k[j] >= from) f(k[j], i + j);
+    });
   }
 
   struct Cut {
@@ -278,22 +311,23 @@ struct Row {
   };
 
   // The lowest-ranked element whose weight ranked above is at most the target, among
-  // keys in [klo, kmax]; keys of `alone` count once, with weight `alone_w` (nothing
-  // when 0). COUNT: weights 1 and target `bound`; else masses and target bound * total.
-  template <bool COUNT>
-  __device__ Cut select(uint32_t klo, double bound, uint32_t alone, double alone_w) {
+  // keys in [klo, khi], with weight `base` ranked above all of them; keys of `alone`
+  // count once, with weight `alone_w` (nothing when 0). COUNT: weights 1. REL: the target
+  // is `bound` times the keys' weight, else `bound`.
+  template <bool COUNT, bool REL>
+  __device__ Cut select(uint32_t klo, uint32_t khi, double base, double bound, uint32_t alone, double alone_w) {
     double* hist = reinterpret_cast<double*>(work);  // [bin][thread]
-    const uint32_t span = kmax - klo;
+    const uint32_t span = khi - klo;
     const int bits = 32 - __clz(span | 1u);
     uint32_t prefix = 0;
-    Cut c{klo, 0.0, 0.0, bound};
+    Cut c{klo, base, 0.0, bound};
     bool first_pass = true;
     __syncthreads();
     for (int shift = (bits - 1) / kDigit * kDigit; shift >= 0; shift -= kDigit) {
 #pragma unroll
       for (int b = 0; b < kBins; ++b) hist[b * kThreads + threadIdx.x] = 0.0;
-      each([&](uint32_t k, int) {
-        const uint32_t o = k - klo;  // keys below klo wrap around to far above the span
+      each(klo, [&](uint32_t k, int) {
+        const uint32_t o = k - klo;
         if (o > span || k == alone || (!first_pass && (o >> (shift + kDigit)) != prefix)) return;
         hist[((o >> shift) & (kBins - 1)) * kThreads + threadIdx.x] += COUNT ? 1.0 : weight(k);
       });
@@ -322,7 +356,7 @@ struct Row {
       }
       __syncthreads();
       parity ^= 1;
-      if (first_pass && !COUNT) {
+      if (first_pass && REL) {
         double z = 0.0;
         for (int b = kBins - 1; b >= 0; --b) z += sh->tot[b];
         c.target = bound * z;
@@ -342,45 +376,21 @@ struct Row {
     return c;
   }
 
-  // This CTA's histogram: counts, or masses as 2^15 w / 2^-bin (bin in units of 1 /
-  // kPerNat nat); for masses the exact sum of the slice's weights comes back.
-  template <bool COUNT>
-  __device__ double histogram() {
-    for (int i = threadIdx.x; i < kHist; i += kThreads) sh->hist[i] = 0;
-    __syncthreads();
-    double z = 0.0;
-    each([&](uint32_t k, int) {
-      if (k == 0) return;
-      const float u = depth(k);
-      if (!COUNT) z += weight(k);
-      if (u < (float)kHist) {
-        const int b = (int)u;
-        atomicAdd(&sh->hist[b], COUNT ? 1u : (uint32_t)(32768.0f * __expf(((float)b - u) * (1.0f / kPerNat))));
-      }
-    });
-    return COUNT ? 0.0 : block_sum(z, sh->scan);
-  }
   // The row's histogram, bins 2 t and 2 t + 1 of thread t (after a cluster_sync).
   __device__ __forceinline__ void row_bins(double (&v)[2]) const {
     v[0] = v[1] = 0.0;
     for (uint32_t r = 0; r < nc; ++r) {
-      v[0] += (double)remote_u32(&sh->hist[2 * threadIdx.x], r);
-      v[1] += (double)remote_u32(&sh->hist[2 * threadIdx.x + 1], r);
+      const uint64_t x = remote_u64(reinterpret_cast<const uint64_t*>(sh->hist) + threadIdx.x, r);
+      v[0] += (double)(uint32_t)x;
+      v[1] += (double)(uint32_t)(x >> 32);
     }
   }
-  // The elements with lo <= depth < hi into this CTA's list; sh->x_count of them, or more than it holds.
-  __device__ void gather(float lo, float hi) {
-    uint64_t* list = reinterpret_cast<uint64_t*>(work);
-    if (threadIdx.x == 0) sh->x_count = 0;
-    __syncthreads();
-    each([&](uint32_t k, int i) {
-      if (k == 0) return;
-      const float u = depth(k);
-      if (u >= lo && u < hi) {
-        const uint32_t at = atomicAdd(&sh->x_count, 1u);
-        if (at < (uint32_t)kList) list[at] = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)(first + i));
-      }
-    });
+  // The element at `position` with key k into this CTA's list; sh->x_count of them, or
+  // more than it holds.
+  __device__ __forceinline__ void put(uint32_t k, int position) {
+    const uint32_t at = atomicAdd(&sh->x_count, 1u);
+    if (at < (uint32_t)kList)
+      reinterpret_cast<uint64_t*>(work)[at] = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)(first + position));
   }
   // CTA 0: all lists, sorted by rank (after a cluster_sync); the others are done with
   // theirs at the next one. -1: too many.
@@ -400,6 +410,7 @@ struct Row {
     return (int)total;
   }
 };
+static_assert(kHist * 8 * 4 <= kBins * kThreads * 8, "the copies of the bins share the work area");
 constexpr int kWorkBytes = kBins * kThreads * 8 > kList * 8 * 2 ? kBins * kThreads * 8 : kList * 8 * 2;
 
 template <typename T>
@@ -419,48 +430,80 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   if (tid < kTable) sh.tab[tid] = exp2((double)tid / kTable);
   if (tid == 0) sh.pick = kThreads;
 
-  // the slice as keys, and the largest of them
-  uint32_t kmax = 0;
+  for (int i = tid; i < kHist; i += kThreads) sh.hist[i] = 0;
+  if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = 0xffffffffu, sh.x_top = 0;
+
+  // the slice as keys, and the thread's largest
+  uint32_t tmax = 0;
   constexpr int VE = 16 / (int)sizeof(T);
   const T* base = reinterpret_cast<const T*>(a.logits) + m * a.ld;
   const bool vec = reinterpret_cast<uintptr_t>(base) % 16 == 0 && a.part_len % VE == 0 && a.part_stride % VE == 0;
   int done = 0;
   if (vec) {
-    for (int i = tid * VE; i + VE <= n; i += kThreads * VE) {
-      const int64_t j = lo + i;
-      const int64_t r = a.n_parts == 1 ? 0 : j / a.part_len;
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(base + r * a.part_stride + (j - r * a.part_len)));
-      const T* e = reinterpret_cast<const T*>(&u);
-      uint4 ku;
-      K* ke = reinterpret_cast<K*>(&ku);
+    const int pieces = n / VE;
+    for (int i0 = tid; i0 < pieces; i0 += 4 * kThreads) {
+      uint4 u[4];
 #pragma unroll
-      for (int t = 0; t < VE; ++t) {
-        ke[t] = KO::key(e[t]);
-        kmax = max(kmax, (uint32_t)ke[t]);
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + q * kThreads;
+        if (i < pieces) {
+          const int64_t j = lo + (int64_t)i * VE, r = a.n_parts == 1 ? 0 : j / a.part_len;
+          u[q] = __ldcs(reinterpret_cast<const uint4*>(base + r * a.part_stride + (j - r * a.part_len)));
+        }
       }
-      *reinterpret_cast<uint4*>(keys + i) = ku;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + q * kThreads;
+        if (i < pieces) {
+          u[q] = make_uint4(KO::keys(u[q].x), KO::keys(u[q].y), KO::keys(u[q].z), KO::keys(u[q].w));
+          reinterpret_cast<uint4*>(keys)[i] = u[q];
+          tmax = KO::max_of(tmax, KO::max_of(KO::max_of(u[q].x, u[q].y), KO::max_of(u[q].z, u[q].w)));
+        }
+      }
     }
-    done = n / VE * VE;
+    tmax = KO::max_in(tmax);
+    done = pieces * VE;
   }
   for (int i = done + tid; i < n; i += kThreads) {
-    const int64_t j = lo + i;
-    const int64_t r = a.n_parts == 1 ? 0 : j / a.part_len;
-    const K k = KO::key(base[r * a.part_stride + (j - r * a.part_len)]);
+    const int64_t j = lo + i, r = a.n_parts == 1 ? 0 : j / a.part_len;
+    const K k = key_of<T>(base[r * a.part_stride + (j - r * a.part_len)]);
     keys[i] = k;
-    kmax = max(kmax, (uint32_t)k);
+    tmax = max(tmax, (uint32_t)k);
   }
-  kmax = __reduce_max_sync(0xffffffffu, kmax);
-  if (lane == 0) sh.wmax[warp] = kmax;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) kmax = max(kmax, sh.wmax[w]);
-    sh.x_max = kmax;
+  auto row_max = [&]() {  // the largest key of the row
+    uint32_t v = __reduce_max_sync(0xffffffffu, tmax);
+    if (lane == 0) sh.wmax[warp] = v;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kWarps; ++w) v = max(v, sh.wmax[w]);
+      sh.x_max = v;
+    }
+    cluster_sync();
+    v = 0;
+    for (uint32_t r = 0; r < nc; ++r) v = max(v, remote_u32(&sh.x_max, r));
+    return v;
+  };
+  uint32_t kmax = row_max();
+  if (kmax > KO::kInf) {  // a NaN somewhere: out with them
+    cluster_sync();
+    tmax = 0;
+    for (int i = tid; i < n; i += kThreads) {
+      if (keys[i] > KO::kInf) keys[i] = 0;
+      tmax = max(tmax, (uint32_t)keys[i]);
+    }
+    kmax = row_max();
   }
-  cluster_sync();
-  kmax = 0;
-  for (uint32_t r = 0; r < nc; ++r) kmax = max(kmax, remote_u32(&sh.x_max, r));
-
-  if (kmax == 0) {  // nothing to draw, for every CTA of the row
+  if (kmax == KO::kInf) {  // +inf: its like share everything, as zeros among nothing
+    cluster_sync();
+    const K zero = key_of<T>(from_f32<T>(0.0f));
+    tmax = 0;
+    for (int i = tid; i < n; i += kThreads) {
+      keys[i] = keys[i] == KO::kInf ? zero : (K)0;
+      tmax = max(tmax, (uint32_t)keys[i]);
+    }
+    kmax = row_max();
+  }
+  if (kmax <= KO::kLow) {  // nothing to draw, for every CTA of the row
     if (rank == 0 && tid == 0) a.out[m] = -1;
     cluster_sync();  // no CTA leaves while another reads its shared memory
     return;
@@ -471,7 +514,6 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   double min_p = a.p.min_p ? a.p.min_p[m] : a.p.min_p_all;
   double u = a.random[m];
   const bool greedy = !(temp > 0.0f);
-  if (greedy) top_k = 1;
   if (!(min_p > 0.0)) min_p = 0.0;
   if (min_p > 1.0) min_p = 1.0;
   if (!(u > 0.0)) u = 0.0;
@@ -481,48 +523,64 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   row.keys = keys, row.n = n, row.first = lo, row.sh = &sh, row.work = dyn, row.rank = rank, row.nc = nc, row.parity = 0;
   row.kmax = kmax;
   const float xmax = KO::value(kmax);
-  row.top_inf = xmax == INFINITY;
-  row.xmax = widen(xmax);
-  row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
-  row.scale_t = row.inv_t * (kTable / 0.6931471805599453);
-  row.lowest = kNegligible / row.inv_t;
+  const double inv_t = greedy ? 1.0 : 1.0 / (double)fminf(fmaxf(temp, 1e-30f), 1e30f), c256 = inv_t * (kTable / 0.6931471805599453);
   row.fmax = xmax;
-  row.per_bin = fminf((float)(row.inv_t * kPerNat), 1e30f);
+  row.ch = (float)c256;
+  row.cl = (float)(c256 - (double)row.ch);
+  const double x_low = (double)xmax + kNegligible / inv_t;
+  row.lowest = x_low > -3.4e38 ? (float)x_low : -FLT_MAX;
+  row.per_bin = fminf((float)(inv_t * kPerNat), 1e30f);
 
   // the lowest key that can have weight: a little below max + kNegligible T
-  uint32_t klo = kmax;
-  if (!row.top_inf) {
-    const double x = row.xmax + (kNegligible - 1.0) / row.inv_t;
-    klo = x > -3.0e38 ? KO::key(from_f32<T>((float)(x - fabs(x) * 0x1p-6))) : 1u;
-    if (klo == 0 || klo > kmax) klo = 1u;
-  }
+  const double x_klo = x_low - 1.0 / inv_t;
+  uint32_t klo = x_klo > -3.0e38 ? (uint32_t)key_of<T>(from_f32<T>((float)(x_klo - fabs(x_klo) * 0x1p-6))) : 0u;
+  klo = klo <= KO::kLow ? KO::kLow + 1 : (klo > kmax ? kmax : klo);
 
+  if (greedy) {  // the first index of the largest logit
+    uint32_t at = 0xffffffffu;
+    row.each(kmax, [&](uint32_t, int i) { at = min(at, (uint32_t)(lo + i)); });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) atomicMin(&sh.x_min, at);
+    cluster_sync();
+    if (rank == 0 && tid == 0) {
+      for (uint32_t r = 0; r < nc; ++r) at = min(at, remote_u32(&sh.x_min, r));
+      a.out[m] = at;
+    }
+    cluster_sync();
+    return;
+  }
   const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0f && !greedy;  // a NaN top_p switches it off
   const double p = top_p > 0.0f ? (double)top_p : 0.0;
   // keys above ckey are kept, and the first cties of those at it
   uint32_t ckey = klo, cties = 0xffffffffu;
   bool digits = cut_k || cut_p;
-  // where differences of logits and their bins cannot overflow into one another
-  const bool binned = fabsf(xmax) <= 1e38f && (greedy || temp <= 1e30f);
+  // where a difference of logits that overflows is out of the bins' range in truth, too
+  const bool binned = fabsf(xmax) <= 1e38f;
 
   if (cut_k && top_k <= kListK && binned) {
-    row.template histogram<true>();
+    // The k-th largest of the threads' largest keys has k elements from it on, and few
+    // more when the large ones are spread over the row: a histogram of one key a thread.
+    const float u0 = tmax >= klo ? row.depth(tmax) : (float)kHist;
+    const int bin = u0 < (float)kHist ? (int)u0 : kHist;
+    if (bin < kHist) atomicAdd(&sh.hist[bin], 1u);
     cluster_sync();
     double v[2], before[2];
     row.row_bins(v);
-    if (tid == 0) sh.at = kHist;
     block_scan<2>(v, before, sh.scan);
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)  // the bin that the k-th rank falls into
+    for (int i = 0; i < 2; ++i)  // the bin that the k-th of them falls into
       if (before[i] < (double)top_k && before[i] + v[i] >= (double)top_k) sh.at = 2 * tid + i;
     __syncthreads();
     const uint32_t at = sh.at;
     if (at < kHist) {
-      row.gather(0.0f, (float)(at + 1));
+      if (bin == (int)at) atomicMin(&sh.x_min, tmax);
       cluster_sync();
-      uint32_t total = 0;
+      uint32_t from = 0xffffffffu, total = 0;
+      for (uint32_t r = 0; r < nc; ++r) from = min(from, remote_u32(&sh.x_min, r));
+      row.each(from, [&](uint32_t k, int i) { row.put(k, i); });
+      cluster_sync();
       for (uint32_t r = 0; r < nc; ++r) total += remote_u32(&sh.x_count, r);
+      klo = from;  // at least k elements from here on
       if (total <= (uint32_t)kList) {
         if (rank == 0) {
           uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
@@ -572,8 +630,36 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       }
     }
   } else if (cut_p && !cut_k && binned) {
-    const double zc = row.template histogram<false>();
-    if (tid == 0) sh.x_mass = zc, sh.at = kHist;
+    // this CTA's masses per bin, as 2^15 w / 2^-bin (bin in nats / kPerNat), and the exact sum
+    double zc = 0.0;
+    // (eight copies of a bin, so that lanes with one logit seldom meet)
+    uint32_t* copies = reinterpret_cast<uint32_t*>(dyn);
+    for (int i = tid; i < kHist * 8 / 4; i += kThreads) reinterpret_cast<uint4*>(copies)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    row.pieces(klo, [&](const uint32_t (&k)[Row<T>::PER], int) {
+#pragma unroll
+      for (int j0 = 0; j0 < Row<T>::PER; j0 += 4) {
+        double w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = row.weight(k[j0 + j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          zc += k[j0 + j] >= klo ? w[j] : 0.0;
+          const float d = row.depth(k[j0 + j]);
+          if (k[j0 + j] >= klo && d < (float)kHist) {
+            const int b = (int)d;
+            atomicAdd(&copies[b * 8 + (lane & 7)], (uint32_t)(32768.0f * __expf(((float)b - d) * (1.0f / kPerNat))));
+          }
+        }
+      }
+    });
+    __syncthreads();
+    for (int i = tid; i < kHist; i += kThreads) {
+      const uint4 x = reinterpret_cast<const uint4*>(copies)[2 * i], y = reinterpret_cast<const uint4*>(copies)[2 * i + 1];
+      sh.hist[i] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
+    }
+    zc = block_sum(zc, sh.scan);
+    if (tid == 0) sh.x_mass = zc;
     cluster_sync();
     double z = 0.0;
     for (uint32_t r = 0; r < nc; ++r) z += remote_f64(&sh.x_mass, r);
@@ -582,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     row.row_bins(v);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      v[i] *= 0x1p-15 * exp_tab(-(double)(2 * tid + i), kTable / 0.6931471805599453 / kPerNat, 1.0 / kPerNat, sh.tab);
+      v[i] *= 0x1p-15 * (double)__expf(-(float)(2 * tid + i) * (1.0f / kPerNat));
     block_scan<2>(v, before, sh.scan);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -591,11 +677,21 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     const uint32_t at = sh.at;
     if (at < kHist) {
       const float w0 = at > 0 ? (float)(at - 1) : 0.0f, w1 = (float)(at + 2);
-      row.gather(w0, w1);
       double above = 0.0;
-      row.each([&](uint32_t k, int) {
-        if (k != 0 && row.depth(k) < w0) above += row.weight(k);
+      uint32_t wlo = 0xffffffffu, whi = 0;
+      row.each(klo, [&](uint32_t k, int i) {
+        const float d = row.depth(k);
+        if (d < w0) {
+          above += row.weight(k);
+        } else if (d < w1) {
+          row.put(k, i);
+          wlo = min(wlo, k);
+          whi = max(whi, k);
+        }
       });
+      wlo = __reduce_min_sync(0xffffffffu, wlo);
+      whi = __reduce_max_sync(0xffffffffu, whi);
+      if (lane == 0) atomicMin(&sh.x_min, wlo), atomicMax(&sh.x_top, whi);
       above = block_sum(above, sh.scan);
       if (tid == 0) sh.x_above = above;
       cluster_sync();
@@ -634,6 +730,25 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
         ckey = remote_u32(&sh.x_key, 0);
         cties = keep;
         digits = false;
+      } else {  // too many for the list: the digits of the window alone
+        uint32_t total = 0;
+        double sum = 0.0;
+        wlo = 0xffffffffu, whi = 0;
+        for (uint32_t r = 0; r < nc; ++r) {
+          total += remote_u32(&sh.x_count, r);
+          sum += remote_f64(&sh.x_above, r);
+          wlo = min(wlo, remote_u32(&sh.x_min, r));
+          whi = max(whi, remote_u32(&sh.x_top, r));
+        }
+        if (total > (uint32_t)kList && sum <= target) {
+          const auto c = row.template select<false, false>(wlo, whi, sum, target, 0u, 0.0);
+          if (c.key > wlo || c.base + c.mass > target) {  // the cut is not below the window
+            const double w = row.weight(c.key), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
+            ckey = c.key;
+            cties = (uint32_t)(more < all ? more : all);
+            digits = false;
+          }
+        }
       }
     }
   }
@@ -641,7 +756,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     uint32_t alone = 0;
     double alone_w = 0.0;
     if (cut_k) {
-      const auto c = row.template select<true>(klo, (double)(top_k - 1), 0u, 0.0);
+      const auto c = row.template select<true, false>(klo, kmax, 0.0, (double)(top_k - 1), 0u, 0.0);
       ckey = c.key;
       const double keep = (double)top_k - c.base;  // of c.mass ties
       cties = (uint32_t)(keep < c.mass ? keep : c.mass);
@@ -649,7 +764,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       alone_w = (double)cties * row.weight(ckey);
     }
     if (cut_p) {
-      const auto c = row.template select<false>(ckey, p, alone, alone_w);
+      const auto c = row.template select<false, true>(cut_k ? ckey : klo, kmax, 0.0, p, alone, alone_w);
       const double w = row.weight(c.key);
       const uint32_t all = (uint32_t)rint(c.mass / w);
       const double more = floor((c.target - c.base) / w);
@@ -658,111 +773,132 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     }
   }
 
-  // kept weight above the cut and ties at it, per contiguous segment of a thread
-  // (odd lengths, so that the threads of a warp start in different banks)
-  const int seg = ((n + kThreads - 1) / kThreads) | 1;
+  // kept weight above the cut and ties at it, per contiguous segment of a thread: an odd
+  // number of 16-byte pieces, so that neighbouring threads read from different banks
+  constexpr int PER = Row<T>::PER;
+  const int seg = (((n + PER - 1) / PER + kThreads - 1) / kThreads | 1) * PER;
   const int s0 = min(tid * seg, n), s1 = min(s0 + seg, n);
   double w_tie = row.weight(ckey);
   if (w_tie < min_p) w_tie = 0.0;
   double strict = 0.0;
   uint32_t ties = 0;
-  for (int i = s0; i < s1; ++i) {
-    const uint32_t k = keys[i];
-    if (k > ckey) {
-      const double w = row.weight(k);
-      strict += w >= min_p ? w : 0.0;
-    } else if (k == ckey) {
-      ++ties;
+  for (int i = s0; i < s1; i += PER) {
+    const uint4 piece = *reinterpret_cast<const uint4*>(keys + i);  // the buffer ends with a whole piece
+    if (KO::max_in(KO::max_of(KO::max_of(piece.x, piece.y), KO::max_of(piece.z, piece.w))) < ckey && i + PER <= s1)
+      continue;
+    const K* e = reinterpret_cast<const K*>(&piece);
+#pragma unroll
+    for (int j0 = 0; j0 < PER; j0 += 4) {
+      double w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = row.weight(e[j0 + j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = i + j0 + j < s1;
+        strict += in && e[j0 + j] > ckey && w[j] >= min_p ? w[j] : 0.0;
+        ties += in && e[j0 + j] == ckey ? 1u : 0u;
+      }
     }
   }
-  // ties before each thread (exclusive, in this CTA) and the CTA's sums
+  // ties before each thread (in this CTA) and the CTA's sums
   uint32_t it = ties;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t v = __shfl_up_sync(0xffffffffu, it, o);
     if (lane >= o) it += v;
   }
-  double st = strict;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) st += __shfl_xor_sync(0xffffffffu, st, o);
+  const double strict_all = block_sum(strict, sh.scan);
   if (lane == 31) sh.iscan[warp] = it;
-  if (lane == 0) sh.scan[warp] = st;
   __syncthreads();
-  uint32_t before = it - ties;
-  for (int w = 0; w < warp; ++w) before += sh.iscan[w];
+  uint32_t before = it - ties, ties_all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t v = sh.iscan[w];
+    before += w < warp ? v : 0u;
+    ties_all += v;
+  }
   if (tid == 0) {
-    double s = 0.0;
-    uint32_t t = 0;
-    for (int w = 0; w < kWarps; ++w) s += sh.scan[w], t += sh.iscan[w];
-    sh.x_mass = s;
-    sh.x_ties = t;
+    sh.x_mass = strict_all;
+    sh.x_ties = ties_all;
+    sh.pick = kThreads;
   }
   cluster_sync();
-  // every CTA finds the one that holds the target
-  double off[kMaxCluster + 1];
-  uint32_t my_before = 0, tb = 0;
-  off[0] = 0.0;
-  for (uint32_t r = 0; r < nc; ++r) {
-    const uint32_t t = remote_u32(&sh.x_ties, r);
-    if (r == rank) my_before = tb;
-    const uint32_t kept = tb < cties ? min(t, cties - tb) : 0u;
-    off[r + 1] = off[r] + (remote_f64(&sh.x_mass, r) + (double)kept * w_tie);
-    tb += t;
-  }
-  const double target = u * off[nc];
-  uint32_t owner = 0;
-  for (uint32_t r = 0; r < nc; ++r)
-    if (off[r + 1] > off[r] && off[r] <= target) owner = r;
-  if (owner == rank) {
-    const double local = target - off[rank];
-    before += my_before;
-    const uint32_t mine = before < cties ? min(ties, cties - before) : 0u;
-    const double mass = strict + (double)mine * w_tie;
+  // every CTA finds the one that holds the target: the last one that starts at or before
+  // it (a lane per CTA)
+  double start, all, target;
+  uint32_t owner;
+  {
+    const bool is = lane < (int)nc;
+    const uint32_t t = is ? remote_u32(&sh.x_ties, lane) : 0u;
+    double mass = is ? remote_f64(&sh.x_mass, lane) : 0.0;
+    uint32_t tb = t;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, tb, o);
+      if (lane >= o) tb += v;
+    }
+    tb -= t;  // ties in the CTAs before
+    mass += (double)(tb < cties ? min(t, cties - tb) : 0u) * w_tie;
     double incl = mass;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
       const double v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    __syncthreads();
-    if (lane == 31) sh.scan[warp] = incl;
-    __syncthreads();
-    double wb = 0.0;
-    for (int w = 0; w < warp; ++w) wb += sh.scan[w];
-    double excl = __shfl_up_sync(0xffffffffu, incl, 1);
-    excl = lane == 0 ? wb : wb + excl;
+    double at = __shfl_up_sync(0xffffffffu, incl, 1);
+    if (lane == 0) at = 0.0;
+    all = __shfl_sync(0xffffffffu, incl, nc - 1);
+    start = __shfl_sync(0xffffffffu, at, rank);
+    before += __shfl_sync(0xffffffffu, tb, rank);
+    target = u * all;
+    owner = 31 - __clz(__ballot_sync(0xffffffffu, is && mass > 0.0 && at <= target));
+  }
+  if (owner == rank) {
+    const double local = target - start;
+    const uint32_t mine = before < cties ? min(ties, cties - before) : 0u;
+    double mass[1] = {strict + (double)mine * w_tie}, excl[1];
+    block_scan<1>(mass, excl, sh.scan);
     // the first thread whose running sum passes the target; when rounding lets
     // none pass, the last one with any weight
-    if (wb + incl > local && mass > 0.0) atomicMin(&sh.pick, tid);
+    if (excl[0] + mass[0] > local && mass[0] > 0.0) atomicMin(&sh.pick, tid);
     __syncthreads();
     if (sh.pick == kThreads) {
       __syncthreads();
       if (tid == 0) sh.pick = -1;
       __syncthreads();
-      if (mass > 0.0) atomicMax(&sh.pick, tid);
+      if (mass[0] > 0.0) atomicMax(&sh.pick, tid);
       __syncthreads();
     }
-    if (tid == sh.pick) {
-      double c = excl;
-      int at = s0;
-      uint32_t tie = before;
-      for (int i = s0; i < s1; ++i) {
-        const uint32_t k = keys[i];
-        double w = 0.0;
-        if (k > ckey) {
-          w = row.weight(k);
-          w = w >= min_p ? w : 0.0;
-        } else if (k == ckey) {
-          w = tie < cties ? w_tie : 0.0;
-          ++tie;
+    if (warp == sh.pick / 32) {  // its warp goes through its segment, 32 elements at a time
+      const int from = sh.pick % 32;
+      const int a0 = __shfl_sync(0xffffffffu, s0, from), a1 = __shfl_sync(0xffffffffu, s1, from);
+      double run = __shfl_sync(0xffffffffu, excl[0], from);
+      uint32_t tie = __shfl_sync(0xffffffffu, before, from);
+      int at = a0;
+      for (int i0 = a0; i0 < a1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < a1 ? (uint32_t)keys[i] : 0u;
+        const uint32_t same = __ballot_sync(0xffffffffu, k == ckey);
+        double w = row.weight(k);
+        w = k > ckey && w >= min_p ? w : 0.0;
+        if (k == ckey) w = tie + __popc(same & ((1u << lane) - 1u)) < cties ? w_tie : 0.0;
+        tie += __popc(same);
+        double incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
         }
-        if (w > 0.0) {
-          at = i;
-          c += w;
-          if (c > local) break;
+        const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
+        const uint32_t past = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > local);
+        if (any) at = i0 + 31 - __clz(any);
+        if (past) {
+          at = i0 + __ffs(past) - 1;
+          break;
         }
+        run += __shfl_sync(0xffffffffu, incl, 31);
       }
-      a.out[m] = lo + at;
+      if (lane == 0) a.out[m] = lo + at;
     }
   }
   cluster_sync();  // no CTA leaves while another reads its shared memory
