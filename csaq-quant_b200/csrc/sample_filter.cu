@@ -15,8 +15,8 @@
 // of the key alone (their errors, one per value and of either sign, move a border by
 // some 1e-11), and no sum goes through an atomic: every order is fixed.
 //
-// A cluster of CTAs takes one row and keeps it in shared memory as ordered integer
-// keys: one pass over the logits. What follows depends on the row's settings:
+// A cluster of CTAs takes one row and keeps it in shared memory: one pass over the
+// logits. What follows depends on the row's settings:
 //
 //  list    top-k up to kListK: a histogram of counts over bins of 1/32 nat below the
 //          largest logit says which bins hold the first k ranks; their tokens, little
@@ -49,9 +49,12 @@ constexpr float kPerNat = 32.0f;
 constexpr int kList = 2048;           // tokens that are sorted at most
 constexpr int kListK = 1024;          // ranks that a list may keep
 constexpr int kMaxCluster = 8;
-constexpr int kTable = 256;           // 2^(j / 256)
-constexpr double kNegligible = -50.0;  // exp below this is taken as 0: 2e-22 of the largest weight
+constexpr int kTable = 256;            // 2^(j / 256)
+constexpr double kNegligible = -50.0;  // weights under e^-50, 2e-22 of the largest, count as 0
+constexpr uint32_t kAll = 0xffffffffu;
 static_assert(kBins * 2 == kWarps && kList == 4 * kThreads && kHist == 2 * kThreads, "shares of a thread");
+constexpr int kWorkBytes = kList * 8 * 2;  // two lists; or the bins of the digit passes; or copies of the histogram
+static_assert(kWorkBytes >= kBins * kThreads * 8 && kWorkBytes >= kHist * 8 * 4, "they share the work area");
 
 struct FilterArgs {
   const void* logits;
@@ -63,55 +66,57 @@ struct FilterArgs {
   int chunk;  // elements of a CTA's slice
 };
 
-// Keys order like the logits, -0 and +0 as one value. kLow is -inf's: a key up to it is
-// -inf or a negative NaN's, one above kInf a positive NaN's (those are set to 0 before
-// use). keys(w): of the packed logits of a 32-bit word.
-template <typename T> struct KeyOf;
-template <> struct KeyOf<float> {
-  using K = uint32_t;
-  static constexpr uint32_t kLow = 0x007fffffu, kInf = 0xff800000u;
-  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
-    const int b = __float_as_int(__uint_as_float(w) + 0.0f);
+// Logits of type T as they lie in 32-bit words. Comparisons go by value: -0 and +0 are
+// one, a NaN is under everything. key(v) orders like v in as few bits as T has values.
+template <typename T> struct Logit;
+template <> struct Logit<float> {
+  static constexpr int N = 1;
+  static __device__ __forceinline__ float value(uint32_t w, int) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float largest(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t key(float v) {
+    const int b = __float_as_int(v + 0.0f);
     return (uint32_t)b ^ ((uint32_t)(b >> 31) | 0x80000000u);
   }
-  static __device__ __forceinline__ float value(uint32_t k) {
+  static __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
   }
-  static __device__ __forceinline__ uint32_t max_in(uint32_t k) { return k; }  // of the keys of a word
-  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return max(a, b); }
 };
-struct Key16 {
-  using K = uint16_t;
-  static __device__ __forceinline__ uint32_t ordered(uint32_t w) {
-    return w ^ (((w >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u);
+template <> struct Logit<__nv_bfloat16> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ float value(uint32_t w, int j) {
+    return __uint_as_float(j ? w & 0xffff0000u : w << 16);
   }
-  static __device__ __forceinline__ uint32_t max_in(uint32_t k) { return max(k & 0xffffu, k >> 16); }
-  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
-};
-template <> struct KeyOf<__half> : Key16 {
-  static constexpr uint32_t kLow = 0x03ffu, kInf = 0xfc00u;
-  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
-    const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.0f));
-    return ordered(*reinterpret_cast<const uint32_t*>(&r));
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
-  static __device__ __forceinline__ float value(uint32_t k) {
-    return __half2float(__ushort_as_half((unsigned short)(k & 0x8000u ? k & 0x7fffu : ~k)));
-  }
-};
-template <> struct KeyOf<__nv_bfloat16> : Key16 {
-  static constexpr uint32_t kLow = 0x007fu, kInf = 0xff80u;
-  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
-    const __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.0f));
-    return ordered(*reinterpret_cast<const uint32_t*>(&r));
-  }
-  static __device__ __forceinline__ float value(uint32_t k) {
+  static __device__ __forceinline__ float largest(uint32_t w) { return fmaxf(value(w, 0), value(w, 1)); }
+  static __device__ __forceinline__ uint32_t key(float v) { return Logit<float>::key(v) >> 16; }
+  static __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu) << 16);
   }
 };
-template <typename T>
-__device__ __forceinline__ typename KeyOf<T>::K key_of(T v) {
-  return (typename KeyOf<T>::K)KeyOf<T>::keys(bits_of<T>(v));
-}
+template <> struct Logit<__half> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ float value(uint32_t w, int j) {
+    return __half2float(__ushort_as_half((unsigned short)(j ? w >> 16 : w)));
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float largest(uint32_t w) { return fmaxf(value(w, 0), value(w, 1)); }
+  static __device__ __forceinline__ uint32_t key(float v) {
+    const uint32_t b = __half_as_ushort(__float2half_rn(v + 0.0f));
+    return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  }
+  static __device__ __forceinline__ float of_key(uint32_t k) {
+    return __half2float(__ushort_as_half((unsigned short)(k & 0x8000u ? k & 0x7fffu : ~k)));
+  }
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -133,46 +138,59 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
                : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
   return r;
 }
-__device__ __forceinline__ double remote_f64(const double* p, uint32_t rank) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote(p, rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint64_t remote_u64(const uint64_t* p, uint32_t rank) {
+__device__ __forceinline__ uint64_t remote_u64(const void* p, uint32_t rank) {
   uint64_t v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t remote_u32(const uint32_t* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-
-// a float's value as a double, by bits (subnormals come out near 2^-127, which next to
-// another logit is all the same)
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+// one value of every CTA of the cluster, a lane each; `none` in the other lanes
+__device__ __forceinline__ uint32_t each_u32(const uint32_t* p, uint32_t nc, uint32_t none) {
+  const uint32_t lane = threadIdx.x & 31;
+  return lane < nc ? remote_u32(p, lane) : none;
+}
+__device__ __forceinline__ double each_f64(const double* p, uint32_t nc) {
+  const uint32_t lane = threadIdx.x & 31;
+  return lane < nc ? __longlong_as_double((long long)remote_u64(p, lane)) : 0.0;
+}
+// the sum over the cluster in rank order
+__device__ __forceinline__ double sum_f64(const double* p, uint32_t nc) {
+  const double mine = each_f64(p, nc);
+  double s = 0.0;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) s += __shfl_sync(0xffffffffu, mine, r);
+  return s;
 }
 
 // exp((v - x) / T) for a result of at least exp(kNegligible), with ch + cl = 256 / (T ln 2):
-// table-driven reduction (Tang 1989) in pairs of fp32. (v - x) exactly as d + e, its
-// product with ch + cl as n + f with n whole; exp = 2^(n / 256) (1 + r + r^2 / 2 + r^3 / 6),
-// r = f ln 2 / 256, |r| <= 0.00136. r is good to 2^-34 and so is the bracket; fp64 takes only
-// the last step (measured here at 12000 clocks for 16000 weights a CTA when it took all).
+// table-driven reduction (Tang 1989) in pairs of fp32. (v - x) as d + e, its product
+// with ch + cl as n + f with n whole; exp = 2^(n / 256) (1 + r + r^2 / 2 + r^3 / 6),
+// r = f ln 2 / 256, |r| <= 0.00136. r is good to 2^-34 and so is the bracket; fp64 takes
+// the last step alone. e is 0 for 16-bit logits unless one is under 2^-16 of the other:
+// there it is left out, 2^-25 of the larger.
+template <bool EXACT>
 __device__ __forceinline__ double exp_tab(float v, float x, float ch, float cl, const double* tab) {
-  const float d = v - x, dv = d - v, e = (v - (d - dv)) - (x + dv);
+  const float d = v - x;
   const float zh = d * ch;
-  const float zl = fmaf(e, ch, fmaf(d, cl, fmaf(d, ch, -zh)));
+  float zl = fmaf(d, cl, fmaf(d, ch, -zh));
+  if (EXACT) {
+    const float dv = d - v;
+    zl = fmaf((v - (d - dv)) - (x + dv), ch, zl);
+  }
   const float magic = 12582912.0f;  // 1.5 2^23: the sum's low bits are the rounded integer
   const float t = zh + magic;
-  const int n = __float_as_int(t) - __float_as_int(magic);
+  const int n = __float_as_int(t);  // and those of the magic number, which neither use below sees
   const float r = ((zh - (t - magic)) + zl) * 0.0027076061740622863f;
   const float q = fmaf(r * r, fmaf(r, 1.0f / 6.0f, 0.5f), r);
   const double c = tab[n & (kTable - 1)];
-  const double w = fma(c, widen(q), c);
-  return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
+  const double w = fma(c, (double)q, c);
+  // 2^(n / 256)'s whole part: n's bits from 8 on, into the exponent (from 20 on)
+  return __hiloint2double(__double2hiint(w) + (int)(((uint32_t)n - 0x4b400000u & ~(kTable - 1u)) << 12),
+                          __double2loint(w));
 }
 
 // Static shared memory; what other CTAs read is marked.
@@ -183,14 +201,14 @@ struct Shared {
   double half[kWarps];
   double scan[kWarps];
   uint32_t iscan[kWarps];
-  double x_mass;     // read by others
-  double x_above;    // read by others
-  uint32_t x_ties;   // read by others
-  uint32_t x_max;    // read by others
-  uint32_t x_min, x_top;  // read by others: smallest and largest key of a window, or the first index
-  uint32_t x_count;  // read by others: tokens in this CTA's list
-  uint32_t x_key, x_keep;  // read by others (CTA 0): the cut of a nucleus; x_keep 0: none was found
-  uint32_t wmax[kWarps];
+  double x_mass;            // read by others
+  double x_above;           // read by others
+  uint32_t x_ties;          // read by others
+  uint32_t x_max;           // read by others: the slice's largest logit, as a key
+  uint32_t x_min, x_top;    // read by others: smallest and largest key of a window, or the first index
+  uint32_t x_count;         // read by others: tokens in this CTA's list
+  uint32_t x_key, x_keep;   // read by others (CTA 0): the cut of a nucleus; x_keep 0: none was found
+  float wmax[kWarps];
   int pick;
   uint32_t at;
   __align__(8) uint32_t hist[kHist];  // read by others
@@ -215,8 +233,9 @@ __device__ __forceinline__ double block_scan(const double (&v)[N], double (&befo
   double wb = 0.0, all = 0.0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) wb += warp_sums[w];
-    all += warp_sums[w];
+    const double x = warp_sums[w];
+    if (w < warp) wb += x;
+    all += x;
   }
   double x = __shfl_up_sync(0xffffffffu, incl, 1);
   x = wb + (lane == 0 ? 0.0 : x);
@@ -239,67 +258,100 @@ __device__ __forceinline__ double block_sum(double v, double* warp_sums) {
   return all;
 }
 
-// bitonic sort of n (a power of two, at most kList) in shared memory, largest first
-__device__ __forceinline__ void sort_down(uint64_t* v, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int a = 2 * i - (i & (step - 1)), b = a + step;
-        const uint64_t x = v[a], y = v[b];
-        if ((x < y) == ((a & size) == 0)) v[a] = y, v[b] = x;
+// Bitonic sort of n (a power of two, at most kList) in shared memory, largest first;
+// `spare` is as long. Up to a thread each they stay in registers, and neighbours up to
+// 16 apart meet by shuffles.
+__device__ __forceinline__ void sort_down(uint64_t* v, uint64_t* spare, int n) {
+  __syncthreads();
+  if (n <= kThreads) {
+    const int i = threadIdx.x;
+    uint64_t x = i < n ? v[i] : 0, *to = spare, *other = v;
+    for (int size = 2; size <= n; size <<= 1)
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        uint64_t y;
+        if (step >= 32) {
+          if (i < n) to[i] = x;
+          __syncthreads();
+          y = i < n ? to[i ^ step] : 0;
+          uint64_t* const swap = to;
+          to = other;
+          other = swap;
+        } else {
+          y = __shfl_xor_sync(0xffffffffu, x, step);
+        }
+        const bool want_max = ((i & step) == 0) == ((i & size) == 0);
+        x = (x < y) == want_max ? y : x;
       }
-    }
+    __syncthreads();
+    if (i < n) v[i] = x;
+  } else {
+    for (int size = 2; size <= n; size <<= 1)
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+          const int a = 2 * i - (i & (step - 1)), b = a + step;
+          const uint64_t x = v[a], y = v[b];
+          if ((x < y) == ((a & size) == 0)) v[a] = y, v[b] = x;
+        }
+        __syncthreads();
+      }
+  }
   __syncthreads();
 }
 __device__ __forceinline__ int pow2_from(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
 template <typename T>
 struct Row {
-  using KO = KeyOf<T>;
-  using K = typename KO::K;
-  const K* keys;  // the slice, in index order
+  using L = Logit<T>;
+  static constexpr int PER = 16 / (int)sizeof(T);  // logits of a 16-byte piece
+  const T* logits;  // the slice, in index order
   int n;
   int64_t first;  // index of its first element
   Shared* sh;
-  uint8_t* work;  // kWorkBytes: the bins of the digit passes, or the list
+  uint8_t* work;  // kWorkBytes
   uint32_t rank, nc;
   int parity;
-  float fmax, ch, cl, lowest, per_bin;  // largest logit, 256 / (T ln 2), the lowest logit with weight, bins
-  uint32_t kmax;
+  float fmax, ch, cl, per_bin;  // largest logit, 256 / (T ln 2), bins per unit
 
-  // (no branch: the weights of a piece are computed side by side)
-  __device__ __forceinline__ double weight(uint32_t k) const {
-    const float v = KO::value(k);
-    const double w = exp_tab(v, fmax, ch, cl, sh->tab);
-    return v >= lowest ? w : 0.0;
+  // (no branch: the weights of a piece are computed side by side; what lies under the
+  // lowest logit with weight is for the caller to leave out)
+  __device__ __forceinline__ double weight(float v) const {
+    return exp_tab<sizeof(T) == 4>(v, fmax, ch, cl, sh->tab);
   }
-  // bins below the largest logit, in exact order of the keys; kHist and more: none
-  __device__ __forceinline__ float depth(uint32_t k) const { return (fmax - KO::value(k)) * per_bin; }
+  // bins below the largest logit, in the order of the logits; kHist and more: none
+  __device__ __forceinline__ float depth(float v) const { return (fmax - v) * per_bin; }
 
-  static constexpr int PER = 16 / (int)sizeof(K);  // keys of a 16-byte piece
-  // f(keys, position, count) over 16-byte pieces (the last one may hold fewer keys);
-  // pieces without a key from `from` on are passed over
-  template <typename F>
-  __device__ __forceinline__ void pieces(uint32_t from, F f) const {
-    for (int i = threadIdx.x * PER; i < n; i += kThreads * PER) {
-      const uint4 u = *reinterpret_cast<const uint4*>(keys + i);  // the buffer ends with a whole piece
-      const int count = min(PER, n - i);
-      if (KO::max_in(KO::max_of(KO::max_of(u.x, u.y), KO::max_of(u.z, u.w))) < from && count == PER) continue;
-      const K* e = reinterpret_cast<const K*>(&u);
-      uint32_t k[PER];
+  __device__ __forceinline__ static float top_of(const uint4& u) {
+    return L::largest(L::larger(L::larger(u.x, u.y), L::larger(u.z, u.w)));
+  }
+  __device__ __forceinline__ static void values(const uint4& u, float (&v)[PER]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int j = 0; j < PER; ++j) k[j] = j < count ? (uint32_t)e[j] : 0u;
-      f(k, i);
+    for (int j = 0; j < PER; ++j) v[j] = L::value(w[j / L::N], j % L::N);
+  }
+  // f(values, position) over the 16-byte pieces with a logit from `from` on; behind the
+  // slice's end values are NaN
+  template <typename F>
+  __device__ __forceinline__ void pieces(float from, F f) const {
+    for (int i = threadIdx.x * PER; i < n; i += kThreads * PER) {
+      const uint4 u = *reinterpret_cast<const uint4*>(logits + i);  // the buffer ends with a whole piece
+      if (i + PER <= n && !(top_of(u) >= from)) continue;
+      float v[PER];
+      values(u, v);
+      if (i + PER > n) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (i + j >= n) v[j] = __uint_as_float(0x7fffffffu);
+      }
+      f(v, i);
     }
   }
-  // f(key, position) over the keys from `from` (at least 1) on
+  // f(logit, position) over the logits from `from` on
   template <typename F>
-  __device__ __forceinline__ void each(uint32_t from, F f) const {
-    pieces(from, [&](const uint32_t (&k)[PER], int i) {
+  __device__ __forceinline__ void each(float from, F f) const {
+    pieces(from, [&](const float (&v)[PER], int i) {
 #pragma unroll
       for (int j = 0; j < PER; ++j)
-        if (k[j] >= from) f(k[j], i + j);
+        if (v[j] >= from) f(v[j], i + j);
     });
   }
 
@@ -319,6 +371,7 @@ struct Row {
     double* hist = reinterpret_cast<double*>(work);  // [bin][thread]
     const uint32_t span = khi - klo;
     const int bits = 32 - __clz(span | 1u);
+    const float from = L::of_key(klo);
     uint32_t prefix = 0;
     Cut c{klo, base, 0.0, bound};
     bool first_pass = true;
@@ -326,10 +379,10 @@ struct Row {
     for (int shift = (bits - 1) / kDigit * kDigit; shift >= 0; shift -= kDigit) {
 #pragma unroll
       for (int b = 0; b < kBins; ++b) hist[b * kThreads + threadIdx.x] = 0.0;
-      each(klo, [&](uint32_t k, int) {
-        const uint32_t o = k - klo;
-        if (o > span || k == alone || (!first_pass && (o >> (shift + kDigit)) != prefix)) return;
-        hist[((o >> shift) & (kBins - 1)) * kThreads + threadIdx.x] += COUNT ? 1.0 : weight(k);
+      each(from, [&](float v, int) {
+        const uint32_t k = L::key(v), o = k - klo;
+        if (o > span || (alone_w != 0.0 && k == alone) || (!first_pass && (o >> (shift + kDigit)) != prefix)) return;
+        hist[((o >> shift) & (kBins - 1)) * kThreads + threadIdx.x] += COUNT ? 1.0 : weight(v);
       });
       if (alone_w != 0.0 && rank == 0 && threadIdx.x == 0) {
         const uint32_t o = alone - klo;
@@ -349,10 +402,9 @@ struct Row {
       __syncthreads();
       if (threadIdx.x < kBins) sh->red[parity][threadIdx.x] = sh->half[2 * threadIdx.x] + sh->half[2 * threadIdx.x + 1];
       cluster_sync();
-      if (threadIdx.x < kBins) {
-        double s = 0.0;
-        for (uint32_t r = 0; r < nc; ++r) s += remote_f64(&sh->red[parity][threadIdx.x], r);
-        sh->tot[threadIdx.x] = s;
+      if (threadIdx.x < kBins * 32) {  // a warp a bin
+        const double s = sum_f64(&sh->red[parity][threadIdx.x >> 5], nc);
+        if ((threadIdx.x & 31) == 0) sh->tot[threadIdx.x >> 5] = s;
       }
       __syncthreads();
       parity ^= 1;
@@ -378,189 +430,171 @@ struct Row {
 
   // The row's histogram, bins 2 t and 2 t + 1 of thread t (after a cluster_sync).
   __device__ __forceinline__ void row_bins(double (&v)[2]) const {
+    uint64_t x[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      x[r] = r < (int)nc ? remote_u64(reinterpret_cast<const uint64_t*>(sh->hist) + threadIdx.x, r) : 0;
     v[0] = v[1] = 0.0;
-    for (uint32_t r = 0; r < nc; ++r) {
-      const uint64_t x = remote_u64(reinterpret_cast<const uint64_t*>(sh->hist) + threadIdx.x, r);
-      v[0] += (double)(uint32_t)x;
-      v[1] += (double)(uint32_t)(x >> 32);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      v[0] += (double)(uint32_t)x[r];
+      v[1] += (double)(uint32_t)(x[r] >> 32);
     }
   }
-  // The element at `position` with key k into this CTA's list; sh->x_count of them, or
-  // more than it holds.
-  __device__ __forceinline__ void put(uint32_t k, int position) {
+  // The element at `position` into this CTA's list; sh->x_count of them, or more than it
+  // holds. Sorted downwards, an entry's order is that of the ranks.
+  __device__ __forceinline__ void put(float v, int position) {
     const uint32_t at = atomicAdd(&sh->x_count, 1u);
     if (at < (uint32_t)kList)
-      reinterpret_cast<uint64_t*>(work)[at] = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)(first + position));
+      reinterpret_cast<uint64_t*>(work)[at] = (uint64_t)Logit<float>::key(v) << 32 | (kAll - (uint32_t)(first + position));
   }
-  // CTA 0: all lists, sorted by rank (after a cluster_sync); the others are done with
-  // theirs at the next one. -1: too many.
-  __device__ int collect() {
+  __device__ __forceinline__ static float logit_of(uint64_t entry) { return Logit<float>::of_key((uint32_t)(entry >> 32)); }
+  // All lists in CTA 0, a warp a CTA; `total` (of all, at most kList). The other CTAs
+  // are done with theirs at the next cluster_sync.
+  __device__ void collect(uint32_t total) {
     uint64_t* list = reinterpret_cast<uint64_t*>(work);
-    uint32_t total = sh->x_count;
-    for (uint32_t r = 1; r < nc; ++r) {
-      const uint32_t c = remote_u32(&sh->x_count, r);
-      if (total + c <= (uint32_t)kList)
-        for (uint32_t i = threadIdx.x; i < c; i += kThreads) list[total + i] = remote_u64(list + i, r);
-      total += c;
+    const uint32_t lane = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const uint32_t c = each_u32(&sh->x_count, nc, 0u);
+    uint32_t before = c;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+      if ((int)lane >= o) before += v;
     }
-    if (total > (uint32_t)kList) return -1;
-    const int size = pow2_from((int)total);
-    for (int i = (int)total + threadIdx.x; i < size; i += kThreads) list[i] = 0;
-    sort_down(list, size);
-    return (int)total;
+    before -= c;
+    const uint32_t mine = __shfl_sync(0xffffffffu, c, r & 7), start = __shfl_sync(0xffffffffu, before, r & 7);
+    if (r > 0 && r < nc)
+      for (uint32_t i = lane; i < mine; i += 32) list[start + i] = remote_u64(list + i, r);
+    for (int i = (int)total + threadIdx.x; i < pow2_from((int)total); i += kThreads) list[i] = 0;
   }
 };
-static_assert(kHist * 8 * 4 <= kBins * kThreads * 8, "the copies of the bins share the work area");
-constexpr int kWorkBytes = kBins * kThreads * 8 > kList * 8 * 2 ? kBins * kThreads * 8 : kList * 8 * 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArgs a) {
-  using KO = KeyOf<T>;
-  using K = typename KO::K;
+  using L = Logit<T>;
+  constexpr int PER = Row<T>::PER;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ Shared sh;
-  pdl_wait();
-  pdl_trigger();
   const uint32_t rank = cluster_rank(), nc = cluster_size();
   const int64_t m = blockIdx.x / nc;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  K* keys = reinterpret_cast<K*>(dyn + kWorkBytes);
+  T* slice = reinterpret_cast<T*>(dyn + kWorkBytes);
   const int64_t lo = (int64_t)rank * a.chunk;
   const int n = (int)(lo >= a.V ? 0 : (a.V - lo < a.chunk ? a.V - lo : a.chunk));
   if (tid < kTable) sh.tab[tid] = exp2((double)tid / kTable);
-  if (tid == 0) sh.pick = kThreads;
-
   for (int i = tid; i < kHist; i += kThreads) sh.hist[i] = 0;
-  if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = 0xffffffffu, sh.x_top = 0;
+  if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = kAll, sh.x_top = 0, sh.x_keep = 0;
+  pdl_wait();
+  pdl_trigger();
 
-  // the slice as keys, and the thread's largest
-  uint32_t tmax = 0;
-  constexpr int VE = 16 / (int)sizeof(T);
+  // the slice, and the thread's largest logit
+  float tmax = -INFINITY;
   const T* base = reinterpret_cast<const T*>(a.logits) + m * a.ld;
-  const bool vec = reinterpret_cast<uintptr_t>(base) % 16 == 0 && a.part_len % VE == 0 && a.part_stride % VE == 0;
+  const bool vec = reinterpret_cast<uintptr_t>(base) % 16 == 0 && a.part_len % PER == 0 && a.part_stride % PER == 0;
   int done = 0;
   if (vec) {
-    const int pieces = n / VE;
-    for (int i0 = tid; i0 < pieces; i0 += 4 * kThreads) {
+    const int whole = n / PER;
+    for (int i0 = tid; i0 < whole; i0 += 4 * kThreads) {
       uint4 u[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int i = i0 + q * kThreads;
-        if (i < pieces) {
-          const int64_t j = lo + (int64_t)i * VE, r = a.n_parts == 1 ? 0 : j / a.part_len;
+        if (i < whole) {
+          const int64_t j = lo + (int64_t)i * PER, r = a.n_parts == 1 ? 0 : j / a.part_len;
           u[q] = __ldcs(reinterpret_cast<const uint4*>(base + r * a.part_stride + (j - r * a.part_len)));
         }
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int i = i0 + q * kThreads;
-        if (i < pieces) {
-          u[q] = make_uint4(KO::keys(u[q].x), KO::keys(u[q].y), KO::keys(u[q].z), KO::keys(u[q].w));
-          reinterpret_cast<uint4*>(keys)[i] = u[q];
-          tmax = KO::max_of(tmax, KO::max_of(KO::max_of(u[q].x, u[q].y), KO::max_of(u[q].z, u[q].w)));
+        if (i < whole) {
+          reinterpret_cast<uint4*>(slice)[i] = u[q];
+          tmax = fmaxf(tmax, Row<T>::top_of(u[q]));
         }
       }
     }
-    tmax = KO::max_in(tmax);
-    done = pieces * VE;
+    done = whole * PER;
   }
   for (int i = done + tid; i < n; i += kThreads) {
     const int64_t j = lo + i, r = a.n_parts == 1 ? 0 : j / a.part_len;
-    const K k = key_of<T>(base[r * a.part_stride + (j - r * a.part_len)]);
-    keys[i] = k;
-    tmax = max(tmax, (uint32_t)k);
+    const T x = base[r * a.part_stride + (j - r * a.part_len)];
+    slice[i] = x;
+    tmax = fmaxf(tmax, to_f32<T>(x));
   }
-  auto row_max = [&]() {  // the largest key of the row
-    uint32_t v = __reduce_max_sync(0xffffffffu, tmax);
+  auto row_max = [&]() {
+    float v = tmax;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (lane == 0) sh.wmax[warp] = v;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) v = max(v, sh.wmax[w]);
-      sh.x_max = v;
+      for (int w = 1; w < kWarps; ++w) v = fmaxf(v, sh.wmax[w]);
+      sh.x_max = Logit<float>::key(v);
     }
     cluster_sync();
-    v = 0;
-    for (uint32_t r = 0; r < nc; ++r) v = max(v, remote_u32(&sh.x_max, r));
-    return v;
+    return Logit<float>::of_key(__reduce_max_sync(0xffffffffu, each_u32(&sh.x_max, nc, 0u)));
   };
-  uint32_t kmax = row_max();
-  if (kmax > KO::kInf) {  // a NaN somewhere: out with them
+  float xmax = row_max();
+  if (xmax == INFINITY) {  // +inf logits share everything: zeros among nothing
     cluster_sync();
-    tmax = 0;
+    tmax = -INFINITY;
     for (int i = tid; i < n; i += kThreads) {
-      if (keys[i] > KO::kInf) keys[i] = 0;
-      tmax = max(tmax, (uint32_t)keys[i]);
+      const bool is = to_f32<T>(slice[i]) == INFINITY;
+      slice[i] = from_f32<T>(is ? 0.0f : -INFINITY);
+      if (is) tmax = 0.0f;
     }
-    kmax = row_max();
+    xmax = row_max();
   }
-  if (kmax == KO::kInf) {  // +inf: its like share everything, as zeros among nothing
-    cluster_sync();
-    const K zero = key_of<T>(from_f32<T>(0.0f));
-    tmax = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      keys[i] = keys[i] == KO::kInf ? zero : (K)0;
-      tmax = max(tmax, (uint32_t)keys[i]);
-    }
-    kmax = row_max();
-  }
-  if (kmax <= KO::kLow) {  // nothing to draw, for every CTA of the row
+  if (xmax == -INFINITY) {  // nothing to draw, for every CTA of the row
     if (rank == 0 && tid == 0) a.out[m] = -1;
     cluster_sync();  // no CTA leaves while another reads its shared memory
     return;
   }
   const float temp = a.p.temperature ? a.p.temperature[m] : a.p.temperature_all;
-  int top_k = a.p.top_k ? a.p.top_k[m] : a.p.top_k_all;
+  const int top_k = a.p.top_k ? a.p.top_k[m] : a.p.top_k_all;
   const float top_p = a.p.top_p ? a.p.top_p[m] : a.p.top_p_all;
-  double min_p = a.p.min_p ? a.p.min_p[m] : a.p.min_p_all;
+  const float min_p = a.p.min_p ? a.p.min_p[m] : a.p.min_p_all;
   double u = a.random[m];
-  const bool greedy = !(temp > 0.0f);
-  if (!(min_p > 0.0)) min_p = 0.0;
-  if (min_p > 1.0) min_p = 1.0;
   if (!(u > 0.0)) u = 0.0;
   if (u >= 1.0) u = 1.0 - 0x1p-53;
 
   Row<T> row;
-  row.keys = keys, row.n = n, row.first = lo, row.sh = &sh, row.work = dyn, row.rank = rank, row.nc = nc, row.parity = 0;
-  row.kmax = kmax;
-  const float xmax = KO::value(kmax);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)fminf(fmaxf(temp, 1e-30f), 1e30f), c256 = inv_t * (kTable / 0.6931471805599453);
+  row.logits = slice, row.n = n, row.first = lo, row.sh = &sh, row.work = dyn, row.rank = rank, row.nc = nc, row.parity = 0;
   row.fmax = xmax;
-  row.ch = (float)c256;
-  row.cl = (float)(c256 - (double)row.ch);
-  const double x_low = (double)xmax + kNegligible / inv_t;
-  row.lowest = x_low > -3.4e38 ? (float)x_low : -FLT_MAX;
-  row.per_bin = fminf((float)(inv_t * kPerNat), 1e30f);
-
-  // the lowest key that can have weight: a little below max + kNegligible T
-  const double x_klo = x_low - 1.0 / inv_t;
-  uint32_t klo = x_klo > -3.0e38 ? (uint32_t)key_of<T>(from_f32<T>((float)(x_klo - fabs(x_klo) * 0x1p-6))) : 0u;
-  klo = klo <= KO::kLow ? KO::kLow + 1 : (klo > kmax ? kmax : klo);
-
-  if (greedy) {  // the first index of the largest logit
-    uint32_t at = 0xffffffffu;
-    row.each(kmax, [&](uint32_t, int i) { at = min(at, (uint32_t)(lo + i)); });
+  if (!(temp > 0.0f)) {  // the first index of the largest logit
+    uint32_t at = kAll;
+    row.each(xmax, [&](float, int i) { at = min(at, (uint32_t)(lo + i)); });
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0) atomicMin(&sh.x_min, at);
     cluster_sync();
-    if (rank == 0 && tid == 0) {
-      for (uint32_t r = 0; r < nc; ++r) at = min(at, remote_u32(&sh.x_min, r));
-      a.out[m] = at;
-    }
+    at = __reduce_min_sync(0xffffffffu, each_u32(&sh.x_min, nc, kAll));
+    if (rank == 0 && tid == 0) a.out[m] = at;
     cluster_sync();
     return;
   }
-  const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0f && !greedy;  // a NaN top_p switches it off
+  const double t64 = fminf(fmaxf(temp, 1e-30f), 1e30f), c256 = kTable / 0.6931471805599453 / t64;
+  row.ch = (float)c256;
+  row.cl = (float)(c256 - (double)row.ch);
+  row.per_bin = fminf((float)((double)kPerNat / t64), 1e30f);
+  // The cut: logits above `cut` are kept, and the first `ties` of those at it. At first
+  // it is the lowest logit with weight, or with min_p times the largest weight.
+  const double limit = (double)xmax + t64 * (min_p > 0.0f ? log(fmin((double)min_p, 1.0)) : kNegligible);
+  float lowest = limit > -3.4e38 ? (float)limit : -FLT_MAX;
+  if (min_p > 0.0f && (double)lowest < limit) lowest = nextafterf(lowest, INFINITY);
+  const float negligible = (double)xmax + t64 * kNegligible > -3.4e38 ? (float)((double)xmax + t64 * kNegligible) : -FLT_MAX;
+  float cut = negligible;
+  uint32_t ties = kAll;
+
+  const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0f;  // a NaN top_p switches it off
   const double p = top_p > 0.0f ? (double)top_p : 0.0;
-  // keys above ckey are kept, and the first cties of those at it
-  uint32_t ckey = klo, cties = 0xffffffffu;
   bool digits = cut_k || cut_p;
   // where a difference of logits that overflows is out of the bins' range in truth, too
   const bool binned = fabsf(xmax) <= 1e38f;
 
   if (cut_k && top_k <= kListK && binned) {
-    // The k-th largest of the threads' largest keys has k elements from it on, and few
-    // more when the large ones are spread over the row: a histogram of one key a thread.
-    const float u0 = tmax >= klo ? row.depth(tmax) : (float)kHist;
+    // The k-th largest of the threads' largest logits has k elements from it on, and few
+    // more when the large ones are spread over the row: a histogram of one logit a thread.
+    const float u0 = tmax >= negligible ? row.depth(tmax) : (float)kHist;
     const int bin = u0 < (float)kHist ? (int)u0 : kHist;
     if (bin < kHist) atomicAdd(&sh.hist[bin], 1u);
     cluster_sync();
@@ -573,21 +607,23 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     __syncthreads();
     const uint32_t at = sh.at;
     if (at < kHist) {
-      if (bin == (int)at) atomicMin(&sh.x_min, tmax);
+      if (bin == (int)at) atomicMin(&sh.x_min, Logit<float>::key(tmax));
       cluster_sync();
-      uint32_t from = 0xffffffffu, total = 0;
-      for (uint32_t r = 0; r < nc; ++r) from = min(from, remote_u32(&sh.x_min, r));
-      row.each(from, [&](uint32_t k, int i) { row.put(k, i); });
+      const float from = Logit<float>::of_key(__reduce_min_sync(0xffffffffu, each_u32(&sh.x_min, nc, kAll)));
+      row.each(from, [&](float x, int i) { row.put(x, i); });
       cluster_sync();
-      for (uint32_t r = 0; r < nc; ++r) total += remote_u32(&sh.x_count, r);
-      klo = from;  // at least k elements from here on
+      const uint32_t total = __reduce_add_sync(0xffffffffu, each_u32(&sh.x_count, nc, 0u));
+      cut = from;  // at least k elements from here on
       if (total <= (uint32_t)kList) {
+        if (rank == 0) row.collect(total);
+        cluster_sync();  // no CTA leaves while another reads its shared memory
         if (rank == 0) {
           uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
-          const int m1 = min(row.collect(), top_k);  // ranks 0 .. m1 - 1 pass top-k
+          sort_down(list, list + kList, pow2_from((int)total));
+          const int m1 = min((int)total, top_k);  // ranks 0 .. m1 - 1 pass top-k
           double w[2], above[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < m1 ? row.weight((uint32_t)(list[2 * tid + i] >> 32)) : 0.0;
+          for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < m1 ? row.weight(Row<T>::logit_of(list[2 * tid + i])) : 0.0;
           const double z = block_scan<2>(w, above, sh.scan);
           double* by_rank = reinterpret_cast<double*>(dyn) + kList;
           if (tid == 0) sh.at = 0;
@@ -598,21 +634,27 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
             if (r >= m1) continue;
             by_rank[r] = w[i];
             // both cuts keep a first part of the ranks, the first rank always
-            if (r == 0 || ((!cut_p || above[i] <= p * z) && w[i] >= min_p)) atomicMax(&sh.at, (uint32_t)r + 1u);
+            if (r == 0 || ((!cut_p || above[i] <= p * z) && Row<T>::logit_of(list[r]) >= lowest)) atomicMax(&sh.at, (uint32_t)r + 1u);
           }
           __syncthreads();
           const int kept = (int)sh.at, size = pow2_from(kept);
           uint64_t mine[2];
+          double moved[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = 2 * tid + i;
             mine[i] = r < kept ? (list[r] << 32 | (uint32_t)r) : 0;  // the low half rises as the index falls
+            moved[i] = r < kept ? by_rank[r] : 0.0;
           }
           __syncthreads();
+          // weights go behind the first kListK places of the second list, which the sort uses
+          by_rank += kListK;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i) {
             if (2 * tid + i < size) list[2 * tid + i] = mine[i];
-          sort_down(list, size);
+            if (2 * tid + i < kept) by_rank[2 * tid + i] = moved[i];
+          }
+          sort_down(list, list + kList, size);
 #pragma unroll
           for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < kept ? by_rank[(uint32_t)list[2 * tid + i]] : 0.0;
           const double mass = block_scan<2>(w, above, sh.scan);
@@ -623,30 +665,29 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
           for (int i = 0; i < 2; ++i)
             if (2 * tid + i < kept && above[i] + w[i] > target) atomicMin(&sh.pick, 2 * tid + i);
           __syncthreads();
-          if (tid == 0) a.out[m] = (int64_t)(0xffffffffu - (uint32_t)(list[sh.pick] >> 32));
+          if (tid == 0) a.out[m] = (int64_t)(kAll - (uint32_t)(list[sh.pick] >> 32));
         }
-        cluster_sync();  // no CTA leaves while another reads its shared memory
         return;
       }
     }
   } else if (cut_p && !cut_k && binned) {
-    // this CTA's masses per bin, as 2^15 w / 2^-bin (bin in nats / kPerNat), and the exact sum
+    // this CTA's masses per bin, as 2^15 w / 2^-bin (bin in nats / kPerNat), and the exact
+    // sum (eight copies of a bin, so that lanes with one logit seldom meet)
     double zc = 0.0;
-    // (eight copies of a bin, so that lanes with one logit seldom meet)
     uint32_t* copies = reinterpret_cast<uint32_t*>(dyn);
     for (int i = tid; i < kHist * 8 / 4; i += kThreads) reinterpret_cast<uint4*>(copies)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    row.pieces(klo, [&](const uint32_t (&k)[Row<T>::PER], int) {
+    row.pieces(negligible, [&](const float (&x)[PER], int) {
 #pragma unroll
-      for (int j0 = 0; j0 < Row<T>::PER; j0 += 4) {
+      for (int j0 = 0; j0 < PER; j0 += 4) {
         double w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = row.weight(k[j0 + j]);
+        for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          zc += k[j0 + j] >= klo ? w[j] : 0.0;
-          const float d = row.depth(k[j0 + j]);
-          if (k[j0 + j] >= klo && d < (float)kHist) {
+          const float d = row.depth(x[j0 + j]);
+          zc += x[j0 + j] >= negligible ? w[j] : 0.0;
+          if (d < (float)kHist) {
             const int b = (int)d;
             atomicAdd(&copies[b * 8 + (lane & 7)], (uint32_t)(32768.0f * __expf(((float)b - d) * (1.0f / kPerNat))));
           }
@@ -661,9 +702,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     zc = block_sum(zc, sh.scan);
     if (tid == 0) sh.x_mass = zc;
     cluster_sync();
-    double z = 0.0;
-    for (uint32_t r = 0; r < nc; ++r) z += remote_f64(&sh.x_mass, r);
-    const double target = p * z;
+    const double target = p * sum_f64(&sh.x_mass, nc);
     double v[2], before[2];
     row.row_bins(v);
 #pragma unroll
@@ -677,16 +716,25 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     const uint32_t at = sh.at;
     if (at < kHist) {
       const float w0 = at > 0 ? (float)(at - 1) : 0.0f, w1 = (float)(at + 2);
+      const float reach = fmaxf(negligible, xmax - (w1 + 1.0f) / row.per_bin);  // under the window, for passing over
       double above = 0.0;
-      uint32_t wlo = 0xffffffffu, whi = 0;
-      row.each(klo, [&](uint32_t k, int i) {
-        const float d = row.depth(k);
-        if (d < w0) {
-          above += row.weight(k);
-        } else if (d < w1) {
-          row.put(k, i);
-          wlo = min(wlo, k);
-          whi = max(whi, k);
+      uint32_t wlo = kAll, whi = 0;
+      row.pieces(reach, [&](const float (&x)[PER], int i) {
+#pragma unroll
+        for (int j0 = 0; j0 < PER; j0 += 4) {
+          double w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float d = row.depth(x[j0 + j]);
+            above += d < w0 ? w[j] : 0.0;
+            if (d >= w0 && d < w1) {
+              row.put(x[j0 + j], i + j0 + j);
+              wlo = min(wlo, L::key(x[j0 + j]));
+              whi = max(whi, L::key(x[j0 + j]));
+            }
+          }
         }
       });
       wlo = __reduce_min_sync(0xffffffffu, wlo);
@@ -695,24 +743,38 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       above = block_sum(above, sh.scan);
       if (tid == 0) sh.x_above = above;
       cluster_sync();
-      if (rank == 0) {
-        uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
-        const int total = row.collect();
-        if (tid == 0) sh.x_keep = 0, sh.at = 0;
-        if (total > 0) {
-          double base = 0.0;
-          for (uint32_t r = 0; r < nc; ++r) base += remote_f64(&sh.x_above, r);
+      const uint32_t total = __reduce_add_sync(0xffffffffu, each_u32(&sh.x_count, nc, 0u));
+      const double start = sum_f64(&sh.x_above, nc);
+      if (total > (uint32_t)kList) {  // too many for the list: the digits of the window alone
+        wlo = __reduce_min_sync(0xffffffffu, each_u32(&sh.x_min, nc, kAll));
+        whi = __reduce_max_sync(0xffffffffu, each_u32(&sh.x_top, nc, 0u));
+        if (start <= target) {
+          const auto c = row.template select<false, false>(wlo, whi, start, target, 0u, 0.0);
+          if (c.key > wlo || c.base + c.mass > target) {  // the cut is not below the window
+            cut = L::of_key(c.key);
+            const double w = row.weight(cut), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
+            ties = (uint32_t)(more < all ? more : all);
+            digits = false;
+          }
+        }
+      } else {
+        if (rank == 0) {
+          uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
+          row.collect(total);
+          sort_down(list, list + kList, pow2_from((int)total));
+          if (tid == 0) sh.at = 0;
           double w[4], before4[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = 4 * tid + i < total ? row.weight((uint32_t)(list[4 * tid + i] >> 32)) : 0.0;
+          for (int i = 0; i < 4; ++i)
+            w[i] = 4 * tid + i < (int)total ? row.weight(Row<T>::logit_of(list[4 * tid + i])) : 0.0;
           const double inside = block_scan<4>(w, before4, sh.scan);
           __syncthreads();
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (4 * tid + i < total && base + before4[i] <= target) atomicMax(&sh.at, 4u * tid + i + 1u);
+            if (4 * tid + i < (int)total && start + before4[i] <= target) atomicMax(&sh.at, 4u * tid + i + 1u);
           __syncthreads();
           const uint32_t kept = sh.at;  // of the list; the cut lies inside it when its ends say so
-          if (kept > 0 && base + inside > target) {
+          if (kept > 0 && start + inside > target) {
             const uint32_t key = (uint32_t)(list[kept - 1] >> 32);
             uint32_t same = 0;
 #pragma unroll
@@ -723,85 +785,65 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
             if (tid == 0) sh.x_key = key;
           }
         }
-      }
-      cluster_sync();
-      const uint32_t keep = remote_u32(&sh.x_keep, 0);
-      if (keep > 0) {
-        ckey = remote_u32(&sh.x_key, 0);
-        cties = keep;
-        digits = false;
-      } else {  // too many for the list: the digits of the window alone
-        uint32_t total = 0;
-        double sum = 0.0;
-        wlo = 0xffffffffu, whi = 0;
-        for (uint32_t r = 0; r < nc; ++r) {
-          total += remote_u32(&sh.x_count, r);
-          sum += remote_f64(&sh.x_above, r);
-          wlo = min(wlo, remote_u32(&sh.x_min, r));
-          whi = max(whi, remote_u32(&sh.x_top, r));
-        }
-        if (total > (uint32_t)kList && sum <= target) {
-          const auto c = row.template select<false, false>(wlo, whi, sum, target, 0u, 0.0);
-          if (c.key > wlo || c.base + c.mass > target) {  // the cut is not below the window
-            const double w = row.weight(c.key), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
-            ckey = c.key;
-            cties = (uint32_t)(more < all ? more : all);
-            digits = false;
-          }
+        cluster_sync();
+        const uint32_t keep = remote_u32(&sh.x_keep, 0);
+        if (keep > 0) {
+          cut = Logit<float>::of_key(remote_u32(&sh.x_key, 0));
+          ties = keep;
+          digits = false;
         }
       }
     }
   }
   if (digits) {
-    uint32_t alone = 0;
+    uint32_t klo = L::key(fmaxf(cut, L::of_key(L::key(cut)))), alone = 0;
+    const uint32_t khi = L::key(xmax);
     double alone_w = 0.0;
+    if (klo > khi) klo = khi;
     if (cut_k) {
-      const auto c = row.template select<true, false>(klo, kmax, 0.0, (double)(top_k - 1), 0u, 0.0);
-      ckey = c.key;
+      const auto c = row.template select<true, false>(klo, khi, 0.0, (double)(top_k - 1), 0u, 0.0);
+      cut = L::of_key(c.key);
       const double keep = (double)top_k - c.base;  // of c.mass ties
-      cties = (uint32_t)(keep < c.mass ? keep : c.mass);
-      alone = ckey;
-      alone_w = (double)cties * row.weight(ckey);
+      ties = (uint32_t)(keep < c.mass ? keep : c.mass);
+      klo = alone = c.key;
+      alone_w = (double)ties * row.weight(cut);
     }
     if (cut_p) {
-      const auto c = row.template select<false, true>(cut_k ? ckey : klo, kmax, 0.0, p, alone, alone_w);
-      const double w = row.weight(c.key);
-      const uint32_t all = (uint32_t)rint(c.mass / w);
-      const double more = floor((c.target - c.base) / w);
-      ckey = c.key;
-      cties = more + 1.0 < (double)all ? (uint32_t)more + 1u : all;
+      const auto c = row.template select<false, true>(klo, khi, 0.0, p, alone, alone_w);
+      cut = L::of_key(c.key);
+      const double w = row.weight(cut), all = rint(c.mass / w), more = floor((c.target - c.base) / w) + 1.0;
+      ties = (uint32_t)(more < all ? more : all);
     }
   }
+  if (min_p > 0.0f && lowest > cut) cut = lowest, ties = kAll;
 
   // kept weight above the cut and ties at it, per contiguous segment of a thread: an odd
   // number of 16-byte pieces, so that neighbouring threads read from different banks
-  constexpr int PER = Row<T>::PER;
   const int seg = (((n + PER - 1) / PER + kThreads - 1) / kThreads | 1) * PER;
   const int s0 = min(tid * seg, n), s1 = min(s0 + seg, n);
-  double w_tie = row.weight(ckey);
-  if (w_tie < min_p) w_tie = 0.0;
+  const double w_tie = row.weight(cut);
   double strict = 0.0;
-  uint32_t ties = 0;
+  uint32_t tied = 0;
   for (int i = s0; i < s1; i += PER) {
-    const uint4 piece = *reinterpret_cast<const uint4*>(keys + i);  // the buffer ends with a whole piece
-    if (KO::max_in(KO::max_of(KO::max_of(piece.x, piece.y), KO::max_of(piece.z, piece.w))) < ckey && i + PER <= s1)
-      continue;
-    const K* e = reinterpret_cast<const K*>(&piece);
+    const uint4 piece = *reinterpret_cast<const uint4*>(slice + i);  // the buffer ends with a whole piece
+    if (i + PER <= s1 && !(Row<T>::top_of(piece) >= cut)) continue;
+    float x[PER];
+    Row<T>::values(piece, x);
 #pragma unroll
     for (int j0 = 0; j0 < PER; j0 += 4) {
       double w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = row.weight(e[j0 + j]);
+      for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bool in = i + j0 + j < s1;
-        strict += in && e[j0 + j] > ckey && w[j] >= min_p ? w[j] : 0.0;
-        ties += in && e[j0 + j] == ckey ? 1u : 0u;
+        strict += in && x[j0 + j] > cut ? w[j] : 0.0;
+        tied += in && x[j0 + j] == cut ? 1u : 0u;
       }
     }
   }
   // ties before each thread (in this CTA) and the CTA's sums
-  uint32_t it = ties;
+  uint32_t it = tied;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t v = __shfl_up_sync(0xffffffffu, it, o);
@@ -810,27 +852,26 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   const double strict_all = block_sum(strict, sh.scan);
   if (lane == 31) sh.iscan[warp] = it;
   __syncthreads();
-  uint32_t before = it - ties, ties_all = 0;
+  uint32_t before = it - tied, tied_all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     const uint32_t v = sh.iscan[w];
     before += w < warp ? v : 0u;
-    ties_all += v;
+    tied_all += v;
   }
   if (tid == 0) {
     sh.x_mass = strict_all;
-    sh.x_ties = ties_all;
+    sh.x_ties = tied_all;
     sh.pick = kThreads;
   }
   cluster_sync();
   // every CTA finds the one that holds the target: the last one that starts at or before
   // it (a lane per CTA)
-  double start, all, target;
+  double start, target;
   uint32_t owner;
   {
-    const bool is = lane < (int)nc;
-    const uint32_t t = is ? remote_u32(&sh.x_ties, lane) : 0u;
-    double mass = is ? remote_f64(&sh.x_mass, lane) : 0.0;
+    const uint32_t t = each_u32(&sh.x_ties, nc, 0u);
+    double mass = each_f64(&sh.x_mass, nc);
     uint32_t tb = t;
 #pragma unroll
     for (int o = 1; o < kMaxCluster; o <<= 1) {
@@ -838,7 +879,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       if (lane >= o) tb += v;
     }
     tb -= t;  // ties in the CTAs before
-    mass += (double)(tb < cties ? min(t, cties - tb) : 0u) * w_tie;
+    mass += (double)(tb < ties ? min(t, ties - tb) : 0u) * w_tie;
     double incl = mass;
 #pragma unroll
     for (int o = 1; o < kMaxCluster; o <<= 1) {
@@ -847,15 +888,14 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     }
     double at = __shfl_up_sync(0xffffffffu, incl, 1);
     if (lane == 0) at = 0.0;
-    all = __shfl_sync(0xffffffffu, incl, nc - 1);
     start = __shfl_sync(0xffffffffu, at, rank);
     before += __shfl_sync(0xffffffffu, tb, rank);
-    target = u * all;
-    owner = 31 - __clz(__ballot_sync(0xffffffffu, is && mass > 0.0 && at <= target));
+    target = u * __shfl_sync(0xffffffffu, incl, nc - 1);
+    owner = 31 - __clz(__ballot_sync(0xffffffffu, lane < (int)nc && mass > 0.0 && at <= target));
   }
   if (owner == rank) {
     const double local = target - start;
-    const uint32_t mine = before < cties ? min(ties, cties - before) : 0u;
+    const uint32_t mine = before < ties ? min(tied, ties - before) : 0u;
     double mass[1] = {strict + (double)mine * w_tie}, excl[1];
     block_scan<1>(mass, excl, sh.scan);
     // the first thread whose running sum passes the target; when rounding lets
@@ -877,11 +917,11 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       int at = a0;
       for (int i0 = a0; i0 < a1; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t k = i < a1 ? (uint32_t)keys[i] : 0u;
-        const uint32_t same = __ballot_sync(0xffffffffu, k == ckey);
-        double w = row.weight(k);
-        w = k > ckey && w >= min_p ? w : 0.0;
-        if (k == ckey) w = tie + __popc(same & ((1u << lane) - 1u)) < cties ? w_tie : 0.0;
+        const float x = i < a1 ? to_f32<T>(slice[i]) : -INFINITY;
+        const uint32_t same = __ballot_sync(0xffffffffu, x == cut);
+        double w = row.weight(x);
+        w = x > cut ? w : 0.0;
+        if (x == cut) w = tie + __popc(same & ((1u << lane) - 1u)) < ties ? w_tie : 0.0;
         tie += __popc(same);
         double incl = w;
 #pragma unroll
@@ -908,10 +948,10 @@ constexpr int kSmemMax = 200 * 1024;  // dynamic, beside the static struct
 
 template <typename T>
 int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
-  constexpr int per = (kSmemMax - kWorkBytes) / (int)sizeof(typename KeyOf<T>::K) / 8 * 8;
+  constexpr int per = (kSmemMax - kWorkBytes) / (int)sizeof(T) / 8 * 8;
   // CTAs of a row: as many as leave two places an SM (by shared memory), and up to 8
   // while the rows alone leave SMs idle
-  constexpr int two = (110 * 1024 - kWorkBytes - (int)sizeof(Shared)) / (int)sizeof(typename KeyOf<T>::K);
+  constexpr int two = (110 * 1024 - kWorkBytes - (int)sizeof(Shared)) / (int)sizeof(T);
   int nc = 1;
   while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * nc <= 148)) nc *= 2;
   const int64_t chunk = ((a.V + nc - 1) / nc + 7) / 8 * 8;
@@ -931,7 +971,7 @@ int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * nc));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kWorkBytes + chunk * sizeof(typename KeyOf<T>::K);
+    cfg.dynamicSmemBytes = kWorkBytes + chunk * sizeof(T);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
