@@ -15,7 +15,9 @@ from .config import CSAQConfig
 from .core import CausalProfiler, apply_csaq, quantize, solve_clique_budget
 from .inference import CSAQInferenceEngine, SpeculativeReport
 from .kernels import CSAQLinear, QuantizedWeight
+from .kvcache import QuantizedKVCache
 from .modeling import CSAQModelForCausalLM
+from .sampling import sample_tokens
 from .utils import build_calibration_data, compute_perplexity, export_csaq_model, generate_csaq_report
 
 __version__ = "0.5.9+b200.0.1"
@@ -23,6 +25,6 @@ __version__ = "0.5.9+b200.0.1"
 __all__ = [
     "CSAQConfig", "CausalProfiler", "apply_csaq", "quantize", "solve_clique_budget",
     "CSAQInferenceEngine", "SpeculativeReport", "CSAQLinear", "QuantizedWeight",
-    "CSAQModelForCausalLM", "build_calibration_data", "compute_perplexity", "export_csaq_model",
+    "CSAQModelForCausalLM", "QuantizedKVCache", "sample_tokens", "build_calibration_data", "compute_perplexity", "export_csaq_model",
     "generate_csaq_report",
 ]

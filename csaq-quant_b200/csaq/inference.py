@@ -13,6 +13,10 @@ Two paths:
 * Other models, and sampling, run the HF forward (whose linears are
   CSAQLinear) in a Python loop with a DynamicCache.
 
+Beyond the reference: ``kv_bits`` (8 or 4) keeps the runtime's KV cache
+quantised, and ``generate(random=...)`` samples one token per step from the
+caller's random numbers under temperature, top_k, top_p and min_p.
+
 Semantics fixed relative to the reference (csaq/inference.py:396-574): the
 verify pass really uses the verify weights (the reference sets an override
 its forward never reads, :225), draft token k is compared with the
@@ -108,7 +112,10 @@ class CSAQInferenceEngine:
     """Self-speculative decoding engine (csaq/inference.py:125-574)."""
 
     def __init__(self, model: nn.Module, causal_map: Dict[str, List[int]], tokenizer: Optional[Any] = None,
-                 verbose: bool = True, tp_group: Any = None) -> None:
+                 verbose: bool = True, tp_group: Any = None, kv_bits: Optional[int] = None) -> None:
+        if kv_bits not in (None, 8, 4):
+            raise ValueError(f"[CSAQ] kv_bits must be 8, 4 or None, got {kv_bits}")
+        self.kv_bits = kv_bits  # quantised KV cache of the decode runtime
         self.model = model
         self.tp_group = tp_group  # torch.distributed group: tensor-parallel decode runtime
         self.causal_map = causal_map
@@ -249,7 +256,7 @@ class CSAQInferenceEngine:
             L = max(max_len, 64)
             L = (L + 63) // 64 * 64
             rt = DecodeRuntime(self.model, max_batch=batch, max_len=L, lookahead=lookahead,
-                               tp_group=self.tp_group)
+                               tp_group=self.tp_group, kv_bits=self.kv_bits)
             self._runtime, self._runtime_key = rt, key
         return rt
 
@@ -287,15 +294,61 @@ class CSAQInferenceEngine:
         self.telemetry["accepted_tokens"] += report.tokens_accepted
         return result.to(input_ids.device), report
 
+    def _generate_from_random(self, input_ids: Optional[torch.Tensor], random: torch.Tensor, max_new_tokens: int,
+                              temperature, top_k, top_p, min_p) -> Tuple[torch.Tensor, SpeculativeReport]:
+        from . import runtime
+        if input_ids is None or input_ids.dim() != 2 or not torch.cuda.is_available() or not runtime.supports(self.model):
+            raise ValueError("[CSAQ] sampling from given random numbers needs the decode runtime: a Llama/Qwen2 model "
+                             "of CSAQLinear layers, a CUDA device and 2-D input_ids")
+        B, P = input_ids.shape
+        if tuple(random.shape) != (B, max_new_tokens):
+            raise ValueError(f"[CSAQ] random must be ({B}, {max_new_tokens}), one number per new token, got "
+                             f"{tuple(random.shape)}")
+        # the lookahead of a runtime that is already there: this path drafts nothing
+        K = self._runtime_key[1] if self._runtime_key is not None and self._runtime_key[0] == B else 1
+        rt = self.runtime(B, P + max_new_tokens + 2 * K + 2, K)
+        ids_dev = input_ids.to(self.device, non_blocking=True)
+        t0 = time.time()
+        with torch.no_grad():
+            rt.reset(ids_dev, max_new_tokens, verify=False)
+            rt.generate_sampled(random, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, verify=False)
+        out = rt.outputs()[:, :max_new_tokens]
+        result = torch.cat([ids_dev, out], dim=1)
+        torch.cuda.synchronize()
+        n = int(out.shape[1]) * B
+        self.telemetry["total_tokens"] += n
+        self.telemetry["accepted_tokens"] += n
+        return result.to(input_ids.device), SpeculativeReport(
+            mode="standard", tokens_generated=n, tokens_accepted=n, draft_calls=max_new_tokens - 1,
+            total_wallclock_s=time.time() - t0)
+
     # ── public API (csaq/inference.py:325-392) ──────────────────────────────
     def generate(self, input_ids: Optional[torch.Tensor] = None, *, speculative: bool = False,
                  lookahead: int = 4, temperature: float = 1.0, top_p: float = 1.0,
                  max_new_tokens: int = 128, **kwargs: Any) -> Tuple[torch.Tensor, SpeculativeReport]:
+        """Generate max_new_tokens tokens after input_ids.
+
+        With random=(batch, max_new_tokens) numbers in [0, 1) every token is
+        drawn by its number under temperature, top_k, top_p and min_p (each a
+        number or one value per sequence), one token per step on the decode
+        runtime; the same numbers give the same tokens."""
+        random = kwargs.pop("random", None)
+        if random is not None:
+            if speculative:
+                raise ValueError("[CSAQ] speculative sampling draws its own numbers (seed=...): random needs "
+                                 "speculative=False")
+            top_k, min_p = kwargs.pop("top_k", 0), kwargs.pop("min_p", 0.0)
+            if kwargs:
+                raise ValueError(f"[CSAQ] not understood beside random: {sorted(kwargs)}")
+            return self._generate_from_random(input_ids, random, max_new_tokens, temperature, top_k, top_p, min_p)
         if input_ids is not None and self._fast_ok(input_ids, temperature, speculative):
             with torch.no_grad():
                 return self._generate_fast(input_ids, speculative and bool(self._hooks), lookahead,
                                            max_new_tokens, temperature=temperature, top_p=top_p,
                                            seed=kwargs.get("seed"))
+        if self.kv_bits is not None:
+            raise ValueError("[CSAQ] kv_bits needs the decode runtime: a Llama/Qwen2 model of CSAQLinear layers, and "
+                             "greedy decoding, speculative sampling or given random numbers")
         if speculative and self._hooks:
             return self._generate_speculative(input_ids, max_new_tokens, lookahead, temperature, top_p)
         self._ensure_draft_state()

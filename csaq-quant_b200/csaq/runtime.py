@@ -24,6 +24,12 @@ over the gathered vocabulary slices.
 Weights: the draft pass reads only the quantised tiers; the verify pass
 reads the tiers without their protected rows plus the fp16 copies of those
 rows, in the same launch (see CSAQLinear.gemv_descriptors).
+
+KV cache: in the model's dtype, or (kv_bits 8 or 4) quantised as it is written,
+csaq.kvcache.QuantizedKVCache per layer. Then the rotation, the quantised write
+and attention over the codes are two launches, and a long prefill chunk reads
+the cache back for torch's fused attention. A token's attention does not depend
+on how many tokens share its step in either form.
 """
 
 from __future__ import annotations
@@ -41,6 +47,8 @@ import torch.nn.functional as F
 from . import _lib
 from ._lib import check, dtype_code, lib, ptr
 from .kernels import CSAQLinear
+from .kvcache import QuantizedKVCache
+from .sampling import sample_params, sample_tokens
 
 # Prefill chunks of at least this many tokens use the tcgen05 GEMM; smaller
 # steps (decode, verify, short prompts) use the GEMV, which is faster there.
@@ -186,9 +194,15 @@ class DecodeRuntime:
     """Decode / self-speculative generation for a quantised Llama/Qwen2 model."""
 
     def __init__(self, model: nn.Module, max_batch: int, max_len: int, lookahead: int = 4,
-                 prefill_chunk: int = 512, tp_group=None):
+                 prefill_chunk: int = 512, tp_group=None, kv_bits: Optional[int] = None,
+                 kv_group: Optional[int] = None):
         if not supports(model):
             raise ValueError("model is not a Llama/Qwen2 decoder with CSAQLinear layers")
+        if kv_bits not in (None, 8, 4):
+            raise ValueError(f"kv_bits must be 8, 4 or None (the model's dtype), got {kv_bits}")
+        if kv_bits is None and kv_group is not None:
+            raise ValueError("kv_group without kv_bits")
+        self.kv_bits = kv_bits
         import torch.distributed as dist
         self.tp_group = tp_group
         self.tp = dist.get_world_size(tp_group) if tp_group is not None else 1
@@ -241,9 +255,18 @@ class DecodeRuntime:
             self.lin.append(mods)
         self.Hq_l, self.Hkv_l, self.I_l = self.Hq // W, self.Hkv // W, self.I // W
         L, B, Hkv, D = self.n_layers, self.B, self.Hkv_l, self.D
-        self.k_cache = torch.zeros(L, B, Hkv, max_len, D, dtype=self.dtype, device=self.dev)
-        self.v_cache = torch.zeros(L, B, Hkv, max_len, D, dtype=self.dtype, device=self.dev)
-        self.tickets = torch.zeros(L, B * Hkv, dtype=torch.int32, device=self.dev)
+        self.kvq: List[QuantizedKVCache] = []  # per layer, with kv_bits
+        self.kv_read: Optional[torch.Tensor] = None  # one layer's keys and values read back, for long prefill chunks
+        if kv_bits is not None:
+            if self.dtype not in (torch.bfloat16, torch.float16):
+                raise ValueError(f"a quantised KV cache needs a bf16 or fp16 model, not {self.dtype}")
+            self.k_cache = self.v_cache = self.tickets = None
+            self.kvq = [QuantizedKVCache(B, Hkv, max_len, D, bits=kv_bits, group_size=kv_group, device=self.dev)
+                        for _ in range(L)]
+        else:
+            self.k_cache = torch.zeros(L, B, Hkv, max_len, D, dtype=self.dtype, device=self.dev)
+            self.v_cache = torch.zeros(L, B, Hkv, max_len, D, dtype=self.dtype, device=self.dev)
+            self.tickets = torch.zeros(L, B * Hkv, dtype=torch.int32, device=self.dev)
         self._rope_tables(inner)
         # generation state
         i32, i64 = torch.int32, torch.int64
@@ -264,6 +287,13 @@ class DecodeRuntime:
         # draft steps' full-vocabulary logits (allocated on first use)
         self.rng = torch.zeros(2, dtype=i64, device=self.dev)
         self.dlog: Optional[torch.Tensor] = None
+        # sampling from given random numbers: this step's numbers and every
+        # sequence's settings (read by the captured step)
+        self.rand = torch.zeros(B, dtype=torch.float32, device=self.dev)
+        self.settings = {"temperature": torch.ones(B, dtype=torch.float32, device=self.dev),
+                         "top_k": torch.zeros(B, dtype=i32, device=self.dev),
+                         "top_p": torch.ones(B, dtype=torch.float32, device=self.dev),
+                         "min_p": torch.zeros(B, dtype=torch.float32, device=self.dev)}
         self.shapes: Dict[int, _Shape] = {}
         # TP combine through peer memory (NVLink), unless CSAQ_TP_EXCHANGE=nccl
         self.p2p: Optional[_P2PExchange] = None
@@ -309,7 +339,10 @@ class DecodeRuntime:
         M = B * S
         mk = lambda *s: torch.zeros(*s, dtype=self.dtype, device=self.dev)
         nq, nkv = Hq * D, Hkv * D
-        part_n = lib().csaq_attention_workspace_floats(B, S, Hq, Hkv, D, self.Lmax)
+        if self.kv_bits is not None:
+            part_n = lib().csaq_kvq_attention_workspace_floats(B, S, Hq, Hkv, D, self.kvq[0].max_len)
+        else:
+            part_n = lib().csaq_attention_workspace_floats(B, S, Hq, Hkv, D, self.Lmax)
         sh = _Shape(S=S, M=M, x=mk(M, H), xn=mk(M, H), qkv=mk(M, nq + 2 * nkv), q_rot=mk(M, nq),
                     attn=mk(M, nq), gu=mk(M, 2 * I), h=mk(M, I), logits=mk(M, self.Vl),
                     part=torch.zeros(max(part_n, 1), dtype=torch.float32, device=self.dev),
@@ -407,6 +440,9 @@ class DecodeRuntime:
         fused scaled-dot-product attention; decode and verify steps to the
         split-key decode kernel with the rotation fused in."""
         qkv, nq, nkv = sh.qkv, self.Hq_l * self.D, self.Hkv_l * self.D
+        if self.kv_bits is not None:
+            self._attention_kvq(li, sh, S, pos, pos_host, scale, st)
+            return
         if pos_host is not None and S >= PREFILL_SDPA_TOKENS:
             check(lib().csaq_rope_kv(qkv.data_ptr(), qkv.stride(0), qkv[:, nq:].data_ptr(), qkv.stride(0),
                                      qkv[:, nq + nkv:].data_ptr(), qkv.stride(0), pos.data_ptr(), self.B, S,
@@ -415,16 +451,7 @@ class DecodeRuntime:
                                      self.v_cache[li].data_ptr(), self.Lmax, self.dt, st), "rope_kv")
             B, Hq, Hkv, D = self.B, self.Hq_l, self.Hkv_l, self.D
             n = pos_host + S
-            q = sh.q_rot.view(B, S, Hq, D).transpose(1, 2)
-            k = self.k_cache[li][:, :, :n]
-            v = self.v_cache[li][:, :, :n]
-            if pos_host == 0:
-                o = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale, enable_gqa=Hq != Hkv)
-            else:  # query i sits at position pos_host + i
-                qi = torch.arange(S, device=self.dev).unsqueeze(1) + pos_host
-                mask = torch.arange(n, device=self.dev).unsqueeze(0) <= qi
-                o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=scale, enable_gqa=Hq != Hkv)
-            sh.attn.view(B, S, Hq, D).copy_(o.transpose(1, 2))
+            self._sdpa(sh, S, self.k_cache[li][:, :, :n], self.v_cache[li][:, :, :n], pos_host, scale)
             return
         # decode / verify / short chunks: RoPE, the cache write and attention in one launch
         check(lib().csaq_decode_attention_rope(qkv.data_ptr(), qkv[:, nq:].data_ptr(), qkv[:, nq + nkv:].data_ptr(),
@@ -433,6 +460,49 @@ class DecodeRuntime:
                                                self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(), self.Lmax,
                                                scale, sh.part.data_ptr(), self.tickets[li].data_ptr(),
                                                sh.attn.data_ptr(), self.dt, st), "attention")
+
+    def _sdpa(self, sh: "_Shape", S: int, k: torch.Tensor, v: torch.Tensor, pos_host: int, scale: float) -> None:
+        """torch's fused attention of the step's rotated queries over k, v
+        (B, Hkv, pos_host + S, D)."""
+        B, Hq, Hkv, D = self.B, self.Hq_l, self.Hkv_l, self.D
+        q = sh.q_rot.view(B, S, Hq, D).transpose(1, 2)
+        if pos_host == 0:
+            o = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale, enable_gqa=Hq != Hkv)
+        else:  # query i sits at position pos_host + i
+            qi = torch.arange(S, device=self.dev).unsqueeze(1) + pos_host
+            mask = torch.arange(k.shape[2], device=self.dev).unsqueeze(0) <= qi
+            o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=scale, enable_gqa=Hq != Hkv)
+        sh.attn.view(B, S, Hq, D).copy_(o.transpose(1, 2))
+
+    def _attention_kvq(self, li: int, sh: "_Shape", S: int, pos: torch.Tensor, pos_host: Optional[int],
+                       scale: float, st: int) -> None:
+        """_attention with a quantised cache: rotation and quantised write, then
+        attention over the codes, or for a long prefill chunk torch's over the
+        positions read back."""
+        c, qkv, nq, nkv, L = self.kvq[li], sh.qkv, self.Hq_l * self.D, self.Hkv_l * self.D, lib()
+        B, Hq, Hkv, D, ld = self.B, self.Hq_l, self.Hkv_l, self.D, sh.qkv.stride(0)
+        check(L.csaq_kvq_write(qkv.data_ptr(), ld, qkv[:, nq:].data_ptr(), ld, qkv[:, nq + nkv:].data_ptr(), ld,
+                               pos.data_ptr(), B, S, Hq, Hkv, D, self.cos.data_ptr(), self.sin.data_ptr(), self.Lmax,
+                               sh.q_rot.data_ptr(), c._ref, self.dt, st), "kvq_write")
+        if pos_host is not None and S >= PREFILL_SDPA_TOKENS:
+            n = pos_host + S
+            if self.kv_read is None or self.kv_read.shape[1] < B * Hkv * n * D:
+                self.kv_read = torch.empty(2, B * Hkv * max(n, self.prefill_chunk) * D, dtype=self.dtype,
+                                           device=self.dev)
+            k, v = (t[: B * Hkv * n * D].view(B, Hkv, n, D) for t in self.kv_read)
+            check(L.csaq_kvq_read(c._ref, B, Hkv, D, 0, n, k.data_ptr(), v.data_ptr(), self.dt, st), "kvq_read")
+            self._sdpa(sh, S, k, v, pos_host, scale)
+            return
+        check(L.csaq_kvq_attention(sh.q_rot.data_ptr(), nq, c._ref, pos.data_ptr(), B, S, Hq, Hkv, D, scale,
+                                   sh.part.data_ptr(), sh.attn.data_ptr(), nq, self.dt, st), "kvq_attention")
+
+    def _attention_launches(self, S: int) -> int:
+        """Own launches of a decode step's attention: one with RoPE fused in, or
+        the quantised write and attention (and the join of its chunks)."""
+        if self.kv_bits is None:
+            return 1
+        n = lib().csaq_kvq_attention_workspace_floats(self.B, S, self.Hq_l, self.Hkv_l, self.D, self.kvq[0].max_len)
+        return 3 if n else 2
 
     @torch.no_grad()
     def step(self, S: int, ids: torch.Tensor, pos: torch.Tensor, verify: bool,
@@ -517,13 +587,13 @@ class DecodeRuntime:
     def kernels_per_step(self, S: int) -> int:
         """Own (libcsaq) kernel launches in one step of up to 16 tokens per
         GEMV launch: per layer 2 RMSNorm, 4 GEMV, RoPE with attention (one
-        launch), SiLU unless the GEMVs run it (and 2 rank-order combines under
+        launch, or two to three with kv_bits), SiLU unless the GEMVs run it (and 2 rank-order combines under
         TP, which through peer memory also run the RMSNorm that follows
         them); plus the final RMSNorm, the lm_head GEMV and the argmax."""
         sh = self._shape(S)
         silu = 0 if self._fused_gate(sh) else 1
         norms = self._norm_launches(sh.M)
-        return self.n_layers * (5 + silu + (2 if self.tp > 1 else 0)) + norms + 2
+        return self.n_layers * (4 + self._attention_launches(S) + silu + (2 if self.tp > 1 else 0)) + norms + 2
 
     def _norm_launches(self, M: int) -> int:
         """Separate RMSNorm launches of one step of M tokens: 2 per layer and
@@ -551,7 +621,10 @@ class DecodeRuntime:
                     else:
                         n += -(-M // 16)
                 silu = 0 if self._fused_gate(sh) else 1  # SiLU, unless inside the GEMVs
-                n += 1 + silu + (2 if self.tp > 1 else 0)  # RoPE (+ SDPA) or fused RoPE + attention
+                # RoPE (+ SDPA) or fused RoPE + attention; with kv_bits the write and the read or attention
+                long = S >= PREFILL_SDPA_TOKENS
+                n += (1 if self.kv_bits is None else 2) if long else self._attention_launches(S)
+                n += silu + (2 if self.tp > 1 else 0)
             n += self._norm_launches(M) + 1  # the RMSNorms and the lm_head
         return n + 1
 
@@ -567,8 +640,8 @@ class DecodeRuntime:
             raise ValueError(f"runtime built for batch {self.B}, got {B}")
         if P + max_new + 2 * self.K + 2 > self.Lmax:
             raise ValueError("prompt + max_new + 2*lookahead + 2 exceeds max_len")
-        self.k_cache.zero_()
-        self.v_cache.zero_()
+        for t in self._cache_buffers():
+            t.zero_()
         self.n_out.zero_()
         self.stats.zero_()
         prompts = prompts.to(self.dev)
@@ -696,7 +769,12 @@ class DecodeRuntime:
 
     def _state(self) -> List[torch.Tensor]:
         return [self.pos0, self.cur_pos, self.next_tok, self.draft, self.vin, self.vt, self.n_new,
-                self.stats, self.remaining, self.out_tokens, self.n_out, self.k_cache, self.v_cache, self.rng]
+                self.stats, self.remaining, self.out_tokens, self.n_out, self.rng, *self._cache_buffers()]
+
+    def _cache_buffers(self) -> List[torch.Tensor]:
+        if self.kv_bits is None:
+            return [self.k_cache, self.v_cache]
+        return [t for c in self.kvq for t in c.buffers()]
 
     def generate_speculative(self, max_new: int, temperature: float = 0.0, top_p: float = 1.0,
                              seed: int = 0) -> int:
@@ -724,6 +802,55 @@ class DecodeRuntime:
         for _ in range(max_new - 1):
             g.replay()
         return max_new - 1
+
+    def _sampled_step(self, verify: bool) -> None:
+        L = lib()
+        st = torch.cuda.current_stream(self.dev).cuda_stream
+        self.step(1, self.next_tok, self.pos0, verify=verify)
+        src, n_parts, pstride, ld, plen = self._logit_parts(1, self.B)
+        params = sample_params(self.B, self.dev, **self.settings)
+        check(L.csaq_sample_filtered(src, n_parts, pstride, ld, plen, self.B, ctypes.byref(params),
+                                     self.rand.data_ptr(), self.argmax_buf.data_ptr(), self.dt, st), "sample_filtered")
+        check(L.csaq_greedy_commit(self.argmax_buf.data_ptr(), self.B, self.pos0.data_ptr(),
+                                   self.out_tokens.data_ptr(), self.n_out.data_ptr(), self.cap,
+                                   self.next_tok.data_ptr(), self.remaining.data_ptr(), st), "commit")
+
+    @torch.no_grad()
+    def generate_sampled(self, random: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                         verify: bool = True) -> int:
+        """Decode after reset(), one token per step, drawn by the caller's numbers:
+        random[b, i] in [0, 1) draws token i of sequence b (token 0 from the
+        prefill's logits). The settings are numbers or one value per sequence
+        (csaq.sampling.sample_tokens). Returns the steps run."""
+        B = self.B
+        if random.dim() != 2 or random.shape[0] != B or random.shape[1] < 1 or not random.is_floating_point():
+            raise ValueError(f"random must hold ({B}, tokens) numbers, got {tuple(random.shape)} {random.dtype}")
+        # the state must have room for the tokens: reset() set max_new
+        n = random.shape[1]
+        room = int(self.remaining.max()) + 1
+        if n > room:
+            raise ValueError(f"{n} random numbers for {room} tokens (max_new of reset)")
+        given = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        sample_params(B, self.dev, **{k: v for k, v in given.items() if not isinstance(v, torch.Tensor)})
+        for k, v in given.items():
+            if isinstance(v, torch.Tensor):
+                if v.shape != (B,):
+                    raise ValueError(f"{k} must be a number or one value per sequence ({B}), got {tuple(v.shape)}")
+                self.settings[k].copy_(v)
+            else:
+                self.settings[k].fill_(v)
+        numbers = random.to(device=self.dev, dtype=torch.float32).t().contiguous()
+        if not hasattr(self, "prefill_logits"):
+            raise RuntimeError("generate_sampled follows reset()")
+        self.rand.copy_(numbers[0])
+        sample_tokens(self.prefill_logits, self.rand, **self.settings, out=self.next_tok)
+        self.out_tokens[:, 0] = self.next_tok
+        if n > 1:
+            g = self._graph("sampled_v" if verify else "sampled_d", lambda: self._sampled_step(verify))
+            for i in range(1, n):
+                self.rand.copy_(numbers[i])
+                g.replay()
+        return n - 1
 
     def outputs(self) -> torch.Tensor:
         n = int(self.n_out.max())
