@@ -256,6 +256,11 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current cudaStream_t of a device: stream_of without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

@@ -21,9 +21,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import CsaqKvqCache, check, dtype_code, lib, ptr, stream_of
+from ._lib import CsaqKvqCache, check, dtype_code, lib, ptr, raw_stream
 
 __all__ = ["KVWorkspace", "QuantizedKVCache", "cache_positions"]
+
+
+_CODES = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 
 
 def cache_positions(n: int) -> int:
@@ -33,7 +36,8 @@ def cache_positions(n: int) -> int:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself when the kernels can read its rows where they are, else a copy."""
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+    ld, one = t.stride()
+    if one != 1 or ld % 8 or ld < t.shape[1] or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:  # a contiguous view at an odd offset
             t = t.clone()
@@ -106,6 +110,8 @@ class QuantizedKVCache:
         self._c = CsaqKvqCache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(), L, bits, self.group_size)
         self._ref = ctypes.byref(self._c)
         self._sizes = {}  # (tokens, heads) -> floats of attend's scratch
+        self._pos_shape = (B,)
+        self._scale = 1.0 / math.sqrt(D)
 
     def buffers(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         return self.k_codes, self.k_params, self.v_codes, self.v_params
@@ -116,35 +122,40 @@ class QuantizedKVCache:
         return self
 
     # ── argument checks shared by the calls ─────────────────────────────────
-    def _tokens(self, t: torch.Tensor, what: str, width: Optional[int] = None) -> int:
-        """Tokens per sequence of a step's matrix t (B*S rows)."""
+    def _tokens(self, t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+        """(tokens per sequence, columns, dtype code) of a step's matrix t (B*S rows)."""
         if t.device != self.device or not t.is_cuda:
             raise RuntimeError(f"csaq-b200: {what} must be on the cache's CUDA device {self.device}, not {t.device}")
-        if t.dtype not in (torch.float16, torch.bfloat16):
+        code = _CODES.get(t.dtype)
+        if code is None:
             raise TypeError(f"csaq-b200: {what} must be float16 or bfloat16, not {t.dtype}")
-        if t.dim() != 2 or t.shape[0] < self.batch or t.shape[0] % self.batch:
-            raise ValueError(f"csaq-b200: {what} needs batch * tokens rows (batch {self.batch}), got {tuple(t.shape)}")
-        if width is not None and t.shape[1] != width:
-            raise ValueError(f"csaq-b200: {what} needs {width} columns, got {t.shape[1]}")
-        return t.shape[0] // self.batch
+        shape = t.shape
+        if len(shape) != 2 or shape[0] < self.batch or shape[0] % self.batch:
+            raise ValueError(f"csaq-b200: {what} needs batch * tokens rows (batch {self.batch}), got {tuple(shape)}")
+        return shape[0] // self.batch, shape[1], code
 
-    def _heads(self, q: torch.Tensor) -> int:
+    def _heads(self, columns: int) -> int:
         step = self.kv_heads * self.head_dim
-        if q.shape[1] < step or q.shape[1] % step:
-            raise ValueError(f"csaq-b200: q needs a multiple of {step} columns (kv_heads * head_dim), got {q.shape[1]}")
-        return q.shape[1] // self.head_dim
+        if columns < step or columns % step:
+            raise ValueError(f"csaq-b200: q needs a multiple of {step} columns (kv_heads * head_dim), got {columns}")
+        return columns // self.head_dim
 
-    def _positions(self, pos0: torch.Tensor) -> None:
-        if pos0.dtype != torch.int32 or pos0.shape != (self.batch,) or pos0.device != self.device \
-                or not pos0.is_contiguous():
+    def _positions(self, pos0: torch.Tensor) -> int:
+        if pos0.dtype is not torch.int32 or pos0.shape != self._pos_shape or pos0.device != self.device \
+                or pos0.stride(0) != 1:
             raise ValueError(f"csaq-b200: pos0 must be {self.batch} contiguous int32 values on {self.device}")
+        return pos0.data_ptr()
 
     def _run(self, fn, what: str, *args) -> None:
-        if self.device.index == torch.cuda.current_device():
-            check(fn(*args), what)
-            return
-        with torch.cuda.device(self.device):
-            check(fn(*args), what)
+        """fn(*args, the current stream of the cache's device), with that device current."""
+        index = self.device.index
+        if index == torch.cuda.current_device():
+            rc = fn(*args, raw_stream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, raw_stream(index))
+        if rc:
+            check(rc, what)
 
     # ── the operators ────────────────────────────────────────────────────────
     def write(self, k: torch.Tensor, v: torch.Tensor, pos0: torch.Tensor, cos: Optional[torch.Tensor] = None,
@@ -158,38 +169,40 @@ class QuantizedKVCache:
         rotated into q_out, which is returned. Positions outside the cache or
         the tables are not stored (their queries pass unrotated)."""
         width = self.kv_heads * self.head_dim
-        S = self._tokens(k, "k", width)
-        if self._tokens(v, "v", width) != S or v.dtype != k.dtype:
-            raise ValueError("csaq-b200: k and v must have one shape and dtype")
-        self._positions(pos0)
+        kind = S, columns, code = self._tokens(k, "k")
+        if self._tokens(v, "v") != kind or columns != width:
+            raise ValueError(f"csaq-b200: k and v must have one dtype and batch * tokens rows of {width} columns")
+        at = self._positions(pos0)
         k, v = _rows(k), _rows(v)
-        Hq, n_rope = 0, 0
+        Hq, n_rope, ldq = 0, 0, 0
         if (cos is None) != (sin is None):
             raise ValueError("csaq-b200: cos and sin come together")
         if cos is not None:
             for t in (cos, sin):
-                if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != self.head_dim or not t.is_contiguous() \
-                        or t.device != self.device or t.shape != cos.shape or t.shape[0] == 0:
+                if t.dtype is not torch.float32 or t.shape != cos.shape or t.dim() != 2 or t.shape[1] != self.head_dim \
+                        or t.device != self.device or not t.is_contiguous() or t.shape[0] == 0:
                     raise ValueError(f"csaq-b200: cos and sin must be contiguous fp32 (positions, {self.head_dim}) "
                                      f"tables on {self.device}")
             n_rope = cos.shape[0]
         if q is not None:
             if cos is None:
                 raise ValueError("csaq-b200: q is only rotated: pass cos and sin with it")
-            if self._tokens(q, "q") != S or q.dtype != k.dtype:
+            Sq, columns, code_q = self._tokens(q, "q")
+            if Sq != S or code_q != code:
                 raise ValueError("csaq-b200: q must have k's rows and dtype")
-            Hq = self._heads(q)
+            Hq = self._heads(columns)
             q = _rows(q)
+            ldq = q.stride(0)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
             elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device \
                     or not q_out.is_contiguous():
                 raise ValueError("csaq-b200: q_out must be contiguous with q's shape and dtype")
         elif q_out is not None:
             raise ValueError("csaq-b200: q_out without q")
-        self._run(lib().csaq_kvq_write, "kvq_write", ptr(q), q.stride(0) if q is not None else 0, k.data_ptr(),
-                  k.stride(0), v.data_ptr(), v.stride(0), pos0.data_ptr(), self.batch, S, Hq, self.kv_heads,
-                  self.head_dim, ptr(cos), ptr(sin), n_rope, ptr(q_out), self._ref, dtype_code(k.dtype), stream_of(k))
+        self._run(lib().csaq_kvq_write, "kvq_write", ptr(q), ldq, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                  at, self.batch, S, Hq, self.kv_heads, self.head_dim, ptr(cos), ptr(sin), n_rope, ptr(q_out),
+                  self._ref, code)
         return q_out
 
     def read(self, start: int, end: int, dtype: torch.dtype = torch.bfloat16,
@@ -210,7 +223,7 @@ class QuantizedKVCache:
         k, v = out
         if end > start:
             self._run(lib().csaq_kvq_read, "kvq_read", self._ref, self.batch, self.kv_heads, self.head_dim, start,
-                      end - start, k.data_ptr(), v.data_ptr(), code, stream_of(k))
+                      end - start, k.data_ptr(), v.data_ptr(), code)
         return k, v
 
     def workspace(self, tokens: int, heads: int) -> KVWorkspace:
@@ -234,22 +247,26 @@ class QuantizedKVCache:
         token (b, s) attends positions 0 .. pos0[b]+s. A token at a negative
         position sees nothing and gets zeros. scale defaults to
         1/sqrt(head_dim). Without a workspace one is allocated for the call."""
-        S = self._tokens(q, "q")
-        Hq = self._heads(q)
-        self._positions(pos0)
+        S, columns, code = self._tokens(q, "q")
+        Hq = self._heads(columns)
+        at = self._positions(pos0)
         q = _rows(q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1 \
-                or out.stride(0) < out.shape[1] or out.stride(0) % 2:
-            raise ValueError("csaq-b200: out must have q's shape and dtype and rows of even stride")
-        if workspace is None:
-            workspace = self.workspace(S, Hq)
-        part = workspace.part
-        if part.device != self.device or part.numel() < self._floats(S, Hq):
-            raise ValueError(f"csaq-b200: the workspace is too small for {S} tokens and {Hq} heads of this cache")
-        self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, pos0.data_ptr(),
-                  self.batch, S, Hq, self.kv_heads, self.head_dim,
-                  float(scale) if scale is not None else 1.0 / math.sqrt(self.head_dim), part.data_ptr(),
-                  out.data_ptr(), out.stride(0), dtype_code(q.dtype), stream_of(q))
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            ldo = columns
+        else:
+            if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1 \
+                    or out.stride(0) < columns or out.stride(0) % 2:
+                raise ValueError("csaq-b200: out must have q's shape and dtype and rows of even stride")
+            ldo = out.stride(0)
+        floats, part = self._floats(S, Hq), None
+        if workspace is not None:
+            part = workspace.part
+            if part.device != self.device or part.numel() < floats:
+                raise ValueError(f"csaq-b200: the workspace is too small for {S} tokens and {Hq} heads of this cache")
+        elif floats:
+            part = torch.empty(floats, dtype=torch.float32, device=self.device)
+        self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, at, self.batch, S, Hq,
+                  self.kv_heads, self.head_dim, self._scale if scale is None else float(scale), ptr(part) if floats else None,
+                  out.data_ptr(), ldo, code)
         return out

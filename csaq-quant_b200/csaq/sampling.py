@@ -16,7 +16,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from ._lib import CsaqSampleParams, check, dtype_code, lib, stream_of
+from ._lib import CsaqSampleParams, check, dtype_code, lib, raw_stream
 
 __all__ = ["sample_tokens", "sample_params"]
 
@@ -83,11 +83,15 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, temperature: Setti
         return out
     if logits.stride(1) != 1 or logits.stride(0) < V:
         logits = logits.contiguous()
-    args = (logits.data_ptr(), 1, 0, logits.stride(0), V, rows, ctypes.byref(params), random.data_ptr(),
-            out.data_ptr(), code, stream_of(logits))
+    def call() -> int:
+        return lib().csaq_sample_filtered(logits.data_ptr(), 1, 0, logits.stride(0), V, rows, ctypes.byref(params),
+                                          random.data_ptr(), out.data_ptr(), code, raw_stream(dev.index))
+
     if dev.index == torch.cuda.current_device():
-        check(lib().csaq_sample_filtered(*args), "sample_filtered")
+        rc = call()
     else:
         with torch.cuda.device(dev):
-            check(lib().csaq_sample_filtered(*args), "sample_filtered")
+            rc = call()
+    if rc:
+        check(rc, "sample_filtered")
     return out
