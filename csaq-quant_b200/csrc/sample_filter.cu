@@ -21,9 +21,10 @@
 //  list    top-k up to kListK: a histogram of counts over bins of 1/32 nat below the
 //          largest logit says which bins hold the first k ranks; their tokens, little
 //          more than k, are gathered in one CTA, sorted, cut and drawn from there.
-//  nucleus top-p alone: a histogram of (approximate) masses says near which bin the cut
-//          lies; the exact mass above three bins and the sorted tokens of the three
-//          give the cut, and a last pass over the row draws under it.
+//  nucleus top-p alone: a histogram of approximate masses says near which bin the cut
+//          lies; one pass sums the exact weight of the row and of what lies above three
+//          bins, whose tokens (no more than a list holds) are narrowed down to the cut,
+//          1 / kHist of their keys' range at a time; the last pass adds those above it.
 //  digits  anything else that cuts, and what the two above hand over (more tokens than
 //          the list holds, a cut out of the bins' range): the cut is found three key
 //          bits at a time; every thread adds its elements into 8 bins of its own, the
@@ -207,7 +208,6 @@ struct Shared {
   uint32_t x_max;           // read by others: the slice's largest logit, as a key
   uint32_t x_min, x_top;    // read by others: smallest and largest key of a window, or the first index
   uint32_t x_count;         // read by others: tokens in this CTA's list
-  uint32_t x_key, x_keep;   // read by others (CTA 0): the cut of a nucleus; x_keep 0: none was found
   float wmax[kWarps];
   int pick;
   uint32_t at;
@@ -328,11 +328,11 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < PER; ++j) v[j] = L::value(w[j / L::N], j % L::N);
   }
-  // f(values, position) over the 16-byte pieces with a logit from `from` on; behind the
-  // slice's end values are NaN
+  // f(values, position) over the 16-byte pieces of [i0, i1) with a logit from `from` on, a
+  // piece every `step` elements; behind the slice's end values are NaN
   template <typename F>
-  __device__ __forceinline__ void pieces(float from, F f) const {
-    for (int i = threadIdx.x * PER; i < n; i += kThreads * PER) {
+  __device__ __forceinline__ void pieces(int i0, int i1, int step, float from, F f) const {
+    for (int i = i0; i < i1; i += step) {
       const uint4 u = *reinterpret_cast<const uint4*>(logits + i);  // the buffer ends with a whole piece
       if (i + PER <= n && !(top_of(u) >= from)) continue;
       float v[PER];
@@ -344,6 +344,11 @@ struct Row {
       }
       f(v, i);
     }
+  }
+  // the same over the whole slice, pieces dealt to the threads in turn
+  template <typename F>
+  __device__ __forceinline__ void pieces(float from, F f) const {
+    pieces(threadIdx.x * PER, n, kThreads * PER, from, f);
   }
   // f(logit, position) over the logits from `from` on
   template <typename F>
@@ -428,17 +433,64 @@ struct Row {
     return c;
   }
 
-  // The row's histogram, bins 2 t and 2 t + 1 of thread t (after a cluster_sync).
-  __device__ __forceinline__ void row_bins(double (&v)[2]) const {
+  // The row's sums of kHist bins, 2 t and 2 t + 1 for thread t (after a cluster_sync).
+  __device__ __forceinline__ void row_bins(const uint64_t* bins, double (&v)[2]) const {
     uint64_t x[kMaxCluster];
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r)
-      x[r] = r < (int)nc ? remote_u64(reinterpret_cast<const uint64_t*>(sh->hist) + threadIdx.x, r) : 0;
+    for (int r = 0; r < kMaxCluster; ++r) x[r] = r < (int)nc ? remote_u64(bins + threadIdx.x, r) : 0;
     v[0] = v[1] = 0.0;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
       v[0] += (double)(uint32_t)x[r];
       v[1] += (double)(uint32_t)(x[r] >> 32);
+    }
+  }
+  // select() among the keys that the CTAs have found (n in this one, at most kList), all in
+  // [klo, khi] and in the order of 1 / kHist of that range at a time. A weight is added
+  // as two integers of 20 bits, relative to the largest (2^-40, under its own error): the
+  // sums do not depend on the order of the atomics.
+  __device__ Cut narrow(const uint32_t* found, int n, uint32_t klo, uint32_t khi, double base, double bound) const {
+    const double unit = weight(L::of_key(khi)) * 0x1p-40, per_unit = 1.0 / unit;
+    uint64_t* bins = reinterpret_cast<uint64_t*>(work + kList * 8);  // low sums of two bins, high sums of two bins
+    Cut c{klo, base, 0.0, bound};
+    for (int flip = 0;; flip ^= 1) {
+      const int shift = max(0, 22 - __clz(khi - klo | 1u));
+      uint32_t* low = reinterpret_cast<uint32_t*>(bins + flip * kHist);
+      for (int i = threadIdx.x; i < kHist; i += kThreads) low[i] = low[kHist + i] = 0;
+      if (threadIdx.x == 0) sh->at = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint32_t o = khi - found[i];
+        if (o > khi - klo) continue;
+        const uint64_t w = __double2ull_rn(fmin(weight(L::of_key(found[i])) * per_unit, 0x1p40));
+        atomicAdd(&low[o >> shift], (uint32_t)w & 0xfffffu);
+        atomicAdd(&low[kHist + (o >> shift)], (uint32_t)(w >> 20));
+      }
+      cluster_sync();
+      double v[2], high[2], before[2];
+      v[0] = v[1] = high[0] = high[1] = 0.0;
+      if (2 * threadIdx.x <= khi - klo >> shift) {
+        row_bins(reinterpret_cast<const uint64_t*>(low), v);
+        row_bins(reinterpret_cast<const uint64_t*>(low + kHist), high);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = (v[i] + high[i] * 0x1p20) * unit;
+      block_scan<2>(v, before, sh->scan);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (v[i] > 0.0 && c.base + before[i] <= bound) atomicMax(&sh->at, 2 * threadIdx.x + i + 1);
+      __syncthreads();
+      const uint32_t pick = sh->at - 1;  // the first bin that holds a key is one
+      if (threadIdx.x == pick / 2) sh->tot[0] = before[pick & 1], sh->tot[1] = v[pick & 1];
+      __syncthreads();
+      c.base += sh->tot[0];
+      c.mass = sh->tot[1];
+      khi -= pick << shift;
+      if (shift == 0) {
+        c.key = khi;
+        return c;
+      }
+      klo = khi - klo >= 1u << shift ? khi - (1u << shift) + 1u : klo;
     }
   }
   // The element at `position` into this CTA's list; sh->x_count of them, or more than it
@@ -483,7 +535,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   const int n = (int)(lo >= a.V ? 0 : (a.V - lo < a.chunk ? a.V - lo : a.chunk));
   if (tid < kTable) sh.tab[tid] = exp2((double)tid / kTable);
   for (int i = tid; i < kHist; i += kThreads) sh.hist[i] = 0;
-  if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = kAll, sh.x_top = 0, sh.x_keep = 0;
+  if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = kAll, sh.x_top = 0;
   pdl_wait();
   pdl_trigger();
 
@@ -527,9 +579,11 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (lane == 0) sh.wmax[warp] = v;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) v = fmaxf(v, sh.wmax[w]);
-      sh.x_max = Logit<float>::key(v);
+    if (warp == 0) {
+      v = sh.wmax[lane % kWarps];
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+      if (lane == 0) sh.x_max = Logit<float>::key(v);
     }
     cluster_sync();
     return Logit<float>::of_key(__reduce_max_sync(0xffffffffu, each_u32(&sh.x_max, nc, 0u)));
@@ -588,6 +642,13 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0f;  // a NaN top_p switches it off
   const double p = top_p > 0.0f ? (double)top_p : 0.0;
   bool digits = cut_k || cut_p;
+  // A thread's contiguous segment for sums in index order: an odd number of 16-byte
+  // pieces, so that neighbouring threads read from different banks.
+  const int seg = (((n + PER - 1) / PER + kThreads - 1) / kThreads | 1) * PER;
+  const int s0 = min(tid * seg, n), s1 = min(s0 + seg, n);
+  double strict = 0.0;  // its weight above the window, when summed
+  float window = 0.0f;  // the window's upper end, in bins
+  bool summed = false;
   // where a difference of logits that overflows is out of the bins' range in truth, too
   const bool binned = fabsf(xmax) <= 1e38f;
 
@@ -599,7 +660,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     if (bin < kHist) atomicAdd(&sh.hist[bin], 1u);
     cluster_sync();
     double v[2], before[2];
-    row.row_bins(v);
+    row.row_bins(reinterpret_cast<const uint64_t*>(sh.hist), v);
     block_scan<2>(v, before, sh.scan);
 #pragma unroll
     for (int i = 0; i < 2; ++i)  // the bin that the k-th of them falls into
@@ -671,27 +732,19 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       }
     }
   } else if (cut_p && !cut_k && binned) {
-    // this CTA's masses per bin, as 2^15 w / 2^-bin (bin in nats / kPerNat), and the exact
-    // sum (eight copies of a bin, so that lanes with one logit seldom meet)
-    double zc = 0.0;
+    // masses per bin (the nearest whole depth), as 2^15 w / e^(-bin / kPerNat), in eight copies, so that
+    // lanes with one logit seldom meet
     uint32_t* copies = reinterpret_cast<uint32_t*>(dyn);
     for (int i = tid; i < kHist * 8 / 4; i += kThreads) reinterpret_cast<uint4*>(copies)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     row.pieces(negligible, [&](const float (&x)[PER], int) {
 #pragma unroll
-      for (int j0 = 0; j0 < PER; j0 += 4) {
-        double w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float d = row.depth(x[j0 + j]);
-          zc += x[j0 + j] >= negligible ? w[j] : 0.0;
-          if (d < (float)kHist) {
-            const int b = (int)d;
-            atomicAdd(&copies[b * 8 + (lane & 7)], (uint32_t)(32768.0f * __expf(((float)b - d) * (1.0f / kPerNat))));
-          }
-        }
+      for (int j = 0; j < PER; ++j) {
+        // sums with 1.5 * 2^23 round, and leave the integer in the low bits
+        const float d = row.depth(x[j]), t = d + 12582912.0f, r = ((t - 12582912.0f) - d) * (1.0f / kPerNat);
+        const float mass = fmaf(fmaf(r, 0.5f, 1.0f) * r, 32768.0f, 32768.0f) + 12582912.0f;
+        if (d < kHist - 1.0f)
+          atomicAdd(&copies[(__float_as_int(t) - 0x4b400000) * 8 + (lane & 7)], __float_as_uint(mass) - 0x4b400000u);
       }
     });
     __syncthreads();
@@ -699,27 +752,26 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       const uint4 x = reinterpret_cast<const uint4*>(copies)[2 * i], y = reinterpret_cast<const uint4*>(copies)[2 * i + 1];
       sh.hist[i] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
     }
-    zc = block_sum(zc, sh.scan);
-    if (tid == 0) sh.x_mass = zc;
     cluster_sync();
-    const double target = p * sum_f64(&sh.x_mass, nc);
     double v[2], before[2];
-    row.row_bins(v);
+    row.row_bins(reinterpret_cast<const uint64_t*>(sh.hist), v);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       v[i] *= 0x1p-15 * (double)__expf(-(float)(2 * tid + i) * (1.0f / kPerNat));
-    block_scan<2>(v, before, sh.scan);
+    const double near = p * block_scan<2>(v, before, sh.scan);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (before[i] <= target && before[i] + v[i] > target) atomicMin(&sh.at, 2u * tid + i);
+      if (before[i] <= near && before[i] + v[i] > near) atomicMin(&sh.at, 2u * tid + i);
     __syncthreads();
     const uint32_t at = sh.at;
     if (at < kHist) {
-      const float w0 = at > 0 ? (float)(at - 1) : 0.0f, w1 = (float)(at + 2);
-      const float reach = fmaxf(negligible, xmax - (w1 + 1.0f) / row.per_bin);  // under the window, for passing over
-      double above = 0.0;
-      uint32_t wlo = kAll, whi = 0;
-      row.pieces(reach, [&](const float (&x)[PER], int i) {
+      // exact weights, of everything and above the window
+      window = at > 0 ? (float)at - 1.5f : 0.0f;
+      const float w1 = (float)at + 1.5f;
+      double zc = 0.0;
+      uint32_t wlo = kAll, whi = 0, *found = reinterpret_cast<uint32_t*>(dyn);  // keys in the window
+      row.pieces(s0, s1, PER, negligible, [&](const float (&x)[PER], int) {
+uint32_t in = 0;  // which of the piece lie in the window
 #pragma unroll
         for (int j0 = 0; j0 < PER; j0 += 4) {
           double w[4];
@@ -728,69 +780,45 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float d = row.depth(x[j0 + j]);
-            above += d < w0 ? w[j] : 0.0;
-            if (d >= w0 && d < w1) {
-              row.put(x[j0 + j], i + j0 + j);
-              wlo = min(wlo, L::key(x[j0 + j]));
-              whi = max(whi, L::key(x[j0 + j]));
-            }
+            zc += x[j0 + j] >= negligible ? w[j] : 0.0;
+            strict += d < window ? w[j] : 0.0;
+            in |= d >= window && d < w1 ? 1u << (j0 + j) : 0u;
           }
+        }
+        if (in) {
+          uint32_t to = atomicAdd(&sh.x_count, (uint32_t)__popc(in));
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (in >> j & 1u) {
+              const uint32_t k = L::key(x[j]);
+              if (to < (uint32_t)kList) found[to] = k;
+              ++to;
+              wlo = min(wlo, k);
+              whi = max(whi, k);
+            }
         }
       });
       wlo = __reduce_min_sync(0xffffffffu, wlo);
       whi = __reduce_max_sync(0xffffffffu, whi);
       if (lane == 0) atomicMin(&sh.x_min, wlo), atomicMax(&sh.x_top, whi);
-      above = block_sum(above, sh.scan);
-      if (tid == 0) sh.x_above = above;
+      zc = block_sum(zc, sh.scan);
+      const double above = block_sum(strict, sh.scan);
+      if (tid == 0) sh.x_mass = zc, sh.x_above = above;
       cluster_sync();
-      const uint32_t total = __reduce_add_sync(0xffffffffu, each_u32(&sh.x_count, nc, 0u));
-      const double start = sum_f64(&sh.x_above, nc);
-      if (total > (uint32_t)kList) {  // too many for the list: the digits of the window alone
-        wlo = __reduce_min_sync(0xffffffffu, each_u32(&sh.x_min, nc, kAll));
-        whi = __reduce_max_sync(0xffffffffu, each_u32(&sh.x_top, nc, 0u));
-        if (start <= target) {
-          const auto c = row.template select<false, false>(wlo, whi, start, target, 0u, 0.0);
-          if (c.key > wlo || c.base + c.mass > target) {  // the cut is not below the window
-            cut = L::of_key(c.key);
-            const double w = row.weight(cut), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
-            ties = (uint32_t)(more < all ? more : all);
-            digits = false;
-          }
-        }
-      } else {
-        if (rank == 0) {
-          uint64_t* list = reinterpret_cast<uint64_t*>(dyn);
-          row.collect(total);
-          sort_down(list, list + kList, pow2_from((int)total));
-          if (tid == 0) sh.at = 0;
-          double w[4], before4[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = 4 * tid + i < (int)total ? row.weight(Row<T>::logit_of(list[4 * tid + i])) : 0.0;
-          const double inside = block_scan<4>(w, before4, sh.scan);
-          __syncthreads();
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (4 * tid + i < (int)total && start + before4[i] <= target) atomicMax(&sh.at, 4u * tid + i + 1u);
-          __syncthreads();
-          const uint32_t kept = sh.at;  // of the list; the cut lies inside it when its ends say so
-          if (kept > 0 && start + inside > target) {
-            const uint32_t key = (uint32_t)(list[kept - 1] >> 32);
-            uint32_t same = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              same += 4u * tid + i < kept && (uint32_t)(list[4 * tid + i] >> 32) == key ? 1u : 0u;
-            same = __reduce_add_sync(0xffffffffu, same);
-            if (lane == 0 && same) atomicAdd(&sh.x_keep, same);
-            if (tid == 0) sh.x_key = key;
-          }
-        }
-        cluster_sync();
-        const uint32_t keep = remote_u32(&sh.x_keep, 0);
-        if (keep > 0) {
-          cut = Logit<float>::of_key(remote_u32(&sh.x_key, 0));
-          ties = keep;
-          digits = false;
+      const uint32_t most = __reduce_max_sync(0xffffffffu, each_u32(&sh.x_count, nc, 0u));
+      const double target = p * sum_f64(&sh.x_mass, nc), start = sum_f64(&sh.x_above, nc);
+      wlo = __reduce_min_sync(0xffffffffu, each_u32(&sh.x_min, nc, kAll));
+      whi = __reduce_max_sync(0xffffffffu, each_u32(&sh.x_top, nc, 0u));
+      if (most > 0 && start <= target) {
+        const auto c = most <= (uint32_t)kList ? row.narrow(found, (int)sh.x_count, wlo, whi, start, target)
+                                               : row.template select<false, false>(wlo, whi, start, target, 0u, 0.0);
+        if (c.key > wlo || c.base + c.mass > target) {  // the cut is not below the window
+          cut = L::of_key(c.key);
+          const double w = row.weight(cut), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
+          ties = (uint32_t)(more < all ? more : all);
+          digits = false, summed = true;
+        } else {
+          cluster_sync();  // the digits take the work area that others may still read
         }
       }
     }
@@ -815,32 +843,41 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       ties = (uint32_t)(more < all ? more : all);
     }
   }
-  if (min_p > 0.0f && lowest > cut) cut = lowest, ties = kAll;
+  if (min_p > 0.0f && lowest > cut) cut = lowest, ties = kAll, summed = false;
 
-  // kept weight above the cut and ties at it, per contiguous segment of a thread: an odd
-  // number of 16-byte pieces, so that neighbouring threads read from different banks
-  const int seg = (((n + PER - 1) / PER + kThreads - 1) / kThreads | 1) * PER;
-  const int s0 = min(tid * seg, n), s1 = min(s0 + seg, n);
+  // kept weight above the cut and ties at it, per segment; where the weight above a window
+  // is summed already, what lies between it and the cut is added
   const double w_tie = row.weight(cut);
-  double strict = 0.0;
   uint32_t tied = 0;
-  for (int i = s0; i < s1; i += PER) {
-    const uint4 piece = *reinterpret_cast<const uint4*>(slice + i);  // the buffer ends with a whole piece
-    if (i + PER <= s1 && !(Row<T>::top_of(piece) >= cut)) continue;
-    float x[PER];
-    Row<T>::values(piece, x);
+  if (summed) {
+    row.pieces(s0, s1, PER, cut, [&](const float (&x)[PER], int) {
+      uint32_t in = 0;
 #pragma unroll
-    for (int j0 = 0; j0 < PER; j0 += 4) {
-      double w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = i + j0 + j < s1;
-        strict += in && x[j0 + j] > cut ? w[j] : 0.0;
-        tied += in && x[j0 + j] == cut ? 1u : 0u;
+      for (int j = 0; j < PER; ++j) {
+        const bool under = row.depth(x[j]) >= window;
+        in |= under && x[j] > cut ? 1u << j : 0u;
+        tied += under && x[j] == cut ? 1u : 0u;
       }
-    }
+      if (in)
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (in >> j & 1u) strict += row.weight(x[j]);
+    });
+  } else {
+    strict = 0.0;
+    row.pieces(s0, s1, PER, cut, [&](const float (&x)[PER], int) {
+#pragma unroll
+      for (int j0 = 0; j0 < PER; j0 += 4) {
+        double w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = row.weight(x[j0 + j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          strict += x[j0 + j] > cut ? w[j] : 0.0;
+          tied += x[j0 + j] == cut ? 1u : 0u;
+        }
+      }
+    });
   }
   // ties before each thread (in this CTA) and the CTA's sums
   uint32_t it = tied;
