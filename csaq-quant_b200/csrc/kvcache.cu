@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(256) kvq_read_kernel(const uint8_t* __restrict
 // Token (b, s) attends keys 0 .. pos0[b] + s. With codes c, zero points z and
 // scales s, a score is s_k (q . c_k - z_k sum q) and an output sum_j (p_j s_j)(c_j - z_j):
 // the scales leave the products, which run on the tensor cores over small integers in
-// fp16, exact, with fp32 sums. They are mma.sync m16n8k16: a key meets at most 32
+// fp16, exact, with fp32 sums. They are mma.sync m16n8k16: a key meets at most 24
 // query rows here, which keeps the tensor pipe under a quarter busy, and the codes go
 // from shared memory through registers straight into operands, where tcgen05 would
 // want them written back first. Keys take the M side of S^T = K q^T and head elements
@@ -1357,10 +1357,14 @@ struct LaunchAttn {
   template <int BITS, int D, int G>
   int run() const {
     const int64_t R = (int64_t)a.S * (a.Hq / a.Hkv);
-    if (R <= 8) return go<BITS, D, G, 1>();
-    if (R <= 16) return go<BITS, D, G, 2>();
-    if (R <= 24) return go<BITS, D, G, 3>();
-    return go<BITS, D, G, 4>();
+    // Rows of a CTA: all of them while that is 24, since each block of rows builds its
+    // operands from the codes anew (16 x 8 heads x 4096 keys, 20 rows: 64 us with 24, 83 with
+    // two blocks of 16, 80 with three of 8), and 16 from then on (16 x 8 x 8192, 32 rows:
+    // 133 us with 16, 181 with 24, 202 with 32, which the registers hold once an SM).
+    // Blocks of 8 when all CTAs then run at once: few CTAs wait for latency (8 heads x 4101
+    // keys, 20 rows: 11.2 us with 8, 14.8 with 24; x 2048, 64 rows: 10.8 with 8, 12.3 with 16).
+    if (R <= 8 || B * a.Hkv * split.n * ((R + 7) / 8) <= kSlots) return go<BITS, D, G, 1>();
+    return R <= 16 || R > 24 ? go<BITS, D, G, 2>() : go<BITS, D, G, 3>();
   }
 };
 

@@ -13,7 +13,7 @@
 // 128k has borders everywhere in [0, 1), and weights or sums in 32 bits would move
 // some of them across u. Sums are therefore fp64, weights good to 2^-32 and a function
 // of the key alone (their errors, one per value and of either sign, move a border by
-// some 1e-11), and no sum goes through an atomic: every order is fixed.
+// some 1e-11), and no sum depends on an order: it is fixed, or the terms are integers.
 //
 // A cluster of CTAs takes one row and keeps it in shared memory: one pass over the
 // logits. What follows depends on the row's settings:
@@ -32,8 +32,7 @@
 //          looks only at the bin that holds the cut.
 //  none    no top-k, no top-p: the last pass alone.
 //
-// The histograms go through integer atomics and only say where to look; the answer
-// never depends on them.
+// The histograms of 1/32 nat only say where to look; the answer never depends on them.
 
 #include <atomic>
 #include <cfloat>
