@@ -343,6 +343,20 @@ def test_attention_independent_of_the_step(bits, D, group):
     assert torch.equal(other[0], together[0])
 
 
+@pytest.mark.parametrize("bits,D,group", [(8, 128, 128), (4, 128, 64), (4, 64, 64), (8, 64, 64)])
+@pytest.mark.parametrize("S", [2, 3, 5])
+def test_attention_independent_of_the_row_blocks(bits, D, group, S):
+    """The same where there are CTAs enough for blocks of 16 and 24 rows: 64 KV heads
+    of 8 query heads, 16, 24 and 40 rows each, against the 8 of a token alone."""
+    B, Hq, Hkv, L = 8, 64, 8, 900
+    c = _filled(B, Hkv, L, D, bits, group, seed=22)
+    q = 3 * torch.randn(B * S, Hq * D, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).to(DEV)
+    pos0 = torch.tensor([0, 1, 15, 130, 511, 513, 700, 894], dtype=torch.int32, device=DEV)
+    together = c.attend(q, pos0).view(B, S, -1)
+    for s in range(S):
+        assert torch.equal(c.attend(q.view(B, S, -1)[:, s].contiguous(), pos0 + s), together[:, s])
+
+
 def test_attention_strides_workspaces_and_repeats():
     """Padded rows of q and out (the padding stays), an own workspace used over and
     over with other lengths and token counts, equal bits."""
