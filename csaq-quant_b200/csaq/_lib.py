@@ -176,6 +176,7 @@ _SIGNATURES = {
     "csaq_kvq_read": (c_int, [ctypes.POINTER(CsaqKvqCache), c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int,
                               c_vp]),
     "csaq_kvq_attention_workspace_floats": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "csaq_kvq_attention_launches": (c_int, [ctypes.POINTER(CsaqKvqCache), c_i64, c_i64, c_i64]),
     "csaq_kvq_attention": (c_int, [c_vp, c_i64, ctypes.POINTER(CsaqKvqCache), c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
                                    ctypes.c_float, c_vp, c_vp, c_i64, c_int, c_vp]),
     "csaq_silu_mul": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]),

@@ -496,13 +496,12 @@ class DecodeRuntime:
         check(L.csaq_kvq_attention(sh.q_rot.data_ptr(), nq, c._ref, pos.data_ptr(), B, S, Hq, Hkv, D, scale,
                                    sh.part.data_ptr(), sh.attn.data_ptr(), nq, self.dt, st), "kvq_attention")
 
-    def _attention_launches(self, S: int) -> int:
+    def _attention_launches(self) -> int:
         """Own launches of a decode step's attention: one with RoPE fused in, or
         the quantised write and attention (and the join of its chunks)."""
         if self.kv_bits is None:
             return 1
-        n = lib().csaq_kvq_attention_workspace_floats(self.B, S, self.Hq_l, self.Hkv_l, self.D, self.kvq[0].max_len)
-        return 3 if n else 2
+        return 1 + lib().csaq_kvq_attention_launches(self.kvq[0]._ref, self.B, self.Hkv_l, self.D)
 
     @torch.no_grad()
     def step(self, S: int, ids: torch.Tensor, pos: torch.Tensor, verify: bool,
@@ -593,7 +592,7 @@ class DecodeRuntime:
         sh = self._shape(S)
         silu = 0 if self._fused_gate(sh) else 1
         norms = self._norm_launches(sh.M)
-        return self.n_layers * (4 + self._attention_launches(S) + silu + (2 if self.tp > 1 else 0)) + norms + 2
+        return self.n_layers * (4 + self._attention_launches() + silu + (2 if self.tp > 1 else 0)) + norms + 2
 
     def _norm_launches(self, M: int) -> int:
         """Separate RMSNorm launches of one step of M tokens: 2 per layer and
@@ -623,7 +622,7 @@ class DecodeRuntime:
                 silu = 0 if self._fused_gate(sh) else 1  # SiLU, unless inside the GEMVs
                 # RoPE (+ SDPA) or fused RoPE + attention; with kv_bits the write and the read or attention
                 long = S >= PREFILL_SDPA_TOKENS
-                n += (1 if self.kv_bits is None else 2) if long else self._attention_launches(S)
+                n += (1 if self.kv_bits is None else 2) if long else self._attention_launches()
                 n += silu + (2 if self.tp > 1 else 0)
             n += self._norm_launches(M) + 1  # the RMSNorms and the lm_head
         return n + 1

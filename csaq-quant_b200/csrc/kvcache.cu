@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(256) kvq_read_kernel(const uint8_t* __restrict
 // A warp takes pairs of 16-key tiles through a ring of its own (16-byte asynchronous
 // copies; no barrier in the loop) and keeps its own softmax state. A CTA's 4 warps
 // join theirs in warp order, then its chunk meets the others in chunk order. Tiles,
-// chunks and joining order depend on key indices and on B Hkv and Lmax alone: a token's
+// chunks and joining order depend on key indices and on B Hkv, Lmax and the bits alone: a token's
 // result does not depend on how many tokens share its step.
 //
 // Bound by HBM for 8 bits (4 x 8 heads x 65536 keys of 128: 94 us, 0.90 of the measured
@@ -1280,21 +1280,24 @@ struct LaunchRead {
   }
 };
 
-// How a cache is cut into chunks, from B * Hkv and Lmax alone (so that a step's token
+// How a cache is cut into chunks, from B * Hkv, Lmax and the bits alone (so that a step's token
 // count does not move the borders). Up to 8 chunks a head are the CTAs of a cluster,
 // fewer when the heads alone are four CTAs for every place on the SMs (chunks even out
 // unequal lengths: 32 sequences x 8 heads of up to 8192 keys, 8-bit, take 60 us in 8
 // chunks, 67 in 2). Where 8 leave SMs without a CTA and the cache is long, one wave
 // of CTAs leaves partials: 1 x 8 heads x 131072 keys, 8-bit, 58 us against 117; at
-// 8192 keys the second kernel costs what the wave gains (11.6 and 11.1 us).
+// 8192 keys the second kernel costs what the wave gains (11.6 and 11.1 us). 4-bit codes,
+// bound by instructions, gain from a full wave at up to 73 heads, too, once they are long:
+// 4 x 8 heads x 65536 keys 69 us against 88, 7 x 8 x 32768 63 against 71, and 4 x 8 x 16384
+// 26 either way; 8-bit ones lose there (4 x 8 x 65536: 102 against 98).
 struct Split {
   int chunk, n;
   bool partial;
 };
 constexpr int64_t kSms = 148, kSlots = 4 * kSms;  // CTAs that run at once (one row block of up to 8 rows)
-Split split_of(int64_t heads, int64_t Lmax) {
+Split split_of(int64_t heads, int64_t Lmax, int bits) {
   Split s;
-  s.partial = heads * kMaxCluster < kSms && Lmax > 8192;
+  s.partial = heads * kMaxCluster < kSms ? Lmax > 8192 : bits == 4 && heads * kMaxCluster < kSlots && Lmax > 16384;
   int64_t n = s.partial ? kSlots / heads : 4 * kSlots / heads;
   if (!s.partial && n > kMaxCluster) n = kMaxCluster;
   if (n < 1) n = 1;
@@ -1408,8 +1411,14 @@ extern "C" int csaq_kvq_read(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv
 extern "C" int64_t csaq_kvq_attention_workspace_floats(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                        int64_t Lmax) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || Lmax <= 0) return -1;
-  const Split split = split_of(B * Hkv, Lmax);
+  const Split split = split_of(B * Hkv, Lmax, 4);  // 8 bits take as much or none
   return split.partial ? B * Hkv * split.n * S * (Hq / Hkv) * (D + 2) : 0;
+}
+
+extern "C" int csaq_kvq_attention_launches(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D) {
+  const int rc = check_cache(cache, B, Hkv, D);
+  if (rc) return rc;
+  return split_of(B * Hkv, cache->Lmax, cache->bits).partial ? 2 : 1;
 }
 
 extern "C" int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cache* cache, const int32_t* pos0,
@@ -1420,7 +1429,7 @@ extern "C" int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cac
   if (!q || !pos0 || !out || S <= 0 || Hq <= 0 || Hq % Hkv || ldq < Hq * D || ldo < Hq * D)
     return CSAQ_ERR_ARG;
   if (dtype != CSAQ_DT_F16 && dtype != CSAQ_DT_BF16) return CSAQ_ERR_ARG;
-  const Split split = split_of(B * Hkv, cache->Lmax);
+  const Split split = split_of(B * Hkv, cache->Lmax, cache->bits);
   if (!part && split.partial) return CSAQ_ERR_ARG;
   if (ldq % 8 || !aligned16(q) || ldo % 2 || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(part) % 8 || S > 65535)
     return CSAQ_ERR_UNSUPPORTED;
@@ -1437,7 +1446,7 @@ extern "C" int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cac
                    (int)cache->Lmax,
                    split.chunk,
                    scale,
-                   part,
+                   split.partial ? part : nullptr,
                    out,
                    ldo,
                    dtype == CSAQ_DT_BF16};

@@ -429,11 +429,14 @@ int csaq_kvq_read(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D
  * token at a negative position sees nothing and its output is 0 (an unused
  * sequence of a batch: pos0[b] = -S). Any S. q needs 16-byte alignment and ldq a
  * multiple of 8; out rows are ldo (even) elements apart. part:
- * csaq_kvq_attention_workspace_floats floats of scratch (8-byte aligned, null when
- * that is 0), rewritten by each call: calls that may overlap on the GPU need one
- * each. A token's result does not depend on S or on the other sequences. */
+ * csaq_kvq_attention_workspace_floats floats of scratch (8-byte aligned; may be null
+ * when that is 0; enough for either width of codes), rewritten by each call: calls
+ * that may overlap on the GPU need one each. A token's result does not depend on S or on the other sequences. */
 int64_t csaq_kvq_attention_workspace_floats(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t Lmax);
+/* Kernels that csaq_kvq_attention launches for B sequences of Hkv heads: 1, or 2
+ * where partials are joined (a negative status for what it refuses). */
+int csaq_kvq_attention_launches(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D);
 int csaq_kvq_attention(const void* q, int64_t ldq, const csaq_kvq_cache* cache, const int32_t* pos0, int64_t B,
                        int64_t S, int64_t Hq, int64_t Hkv, int64_t D, float scale, float* part, void* out,
                        int64_t ldo, int dtype, void* stream);

@@ -94,6 +94,34 @@ def test_speculative_equals_greedy(models, name, B, K, bits):
     assert torch.equal(out[:, 33:].cpu(), rt.outputs()[:, :40].cpu())
 
 
+@pytest.mark.parametrize("name,bits", [("tiny-llama", 8), ("tiny-llama", 4), ("tiny-qwen2-d64", 8)])
+def test_contexts_of_several_chunks(models, name, bits):
+    """400 positions, which attention takes in four chunks of keys: prefill in pieces agrees
+    with prefill in one, the decode steps write nothing but their outputs, and speculation
+    equals greedy decoding."""
+    eng = _engine(models, name, kv_bits=bits)
+    P, n, K = 400, 40, 4
+    rt = eng.runtime(2, P + n + 2 * K + 2, K)
+    prompt = _prompt(2, P, eng.model.config.vocab_size, seed=9).to(DEV)
+    rt.reset(prompt, max_new=n)
+    want = rt.prefill_logits.float()
+    rt.prefill_chunk = 16
+    rt.reset(prompt, max_new=n)
+    rt.prefill_chunk = 512
+    got = rt.prefill_logits.float()
+    assert (got - want).abs().max() / want.abs().max() < 3e-2
+    assert (torch.nn.functional.cosine_similarity(got, want) > 0.999).all()
+    rt.reset(prompt, n, verify=True)
+    held = [[t[:, :, :P].clone() for t in c.buffers()] for c in rt.kvq]
+    weights = {k: v.clone() for k, v in eng.model.state_dict().items()}
+    rt.generate_greedy(n, verify=True)
+    assert all(torch.equal(t[:, :, :P], o) for c, old in zip(rt.kvq, held) for t, o in zip(c.buffers(), old))
+    assert all(torch.equal(v, weights[k]) for k, v in eng.model.state_dict().items())
+    greedy = rt.outputs()[:, :n].cpu()
+    out, _ = eng.generate(prompt.cpu(), speculative=True, lookahead=K, temperature=0.0, max_new_tokens=n)
+    assert torch.equal(out[:, P:].cpu(), greedy)
+
+
 def test_speculative_sampling_runs(models):
     eng = _engine(models, "tiny-llama", kv_bits=8)
     prompt = _prompt(2, 12, eng.model.config.vocab_size, seed=1)

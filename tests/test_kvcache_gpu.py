@@ -381,6 +381,31 @@ def test_attention_strides_workspaces_and_repeats():
                    workspace=big.workspace(4, 8))
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("Hkv", [4, 24, 80])
+def test_scratch_that_is_not_needed(bits, Hkv):
+    """Scratch sized for either width of codes changes nothing where a head's chunks
+    meet in a cluster; 24 heads of a long 4-bit cache leave partials."""
+    D, L, n = 64, 20480, 700
+    c = _cache(1, Hkv, L, D, bits, 64)
+    g = torch.Generator().manual_seed(31)
+    k, v, q = (torch.randn(m, Hkv * D, generator=g).to(torch.float16).to(DEV) for m in (n, n, 1))
+    pos0 = torch.tensor([L - n], dtype=torch.int32, device=DEV)
+    c.write(k, v, pos0)
+    at = torch.tensor([L - 1], dtype=torch.int32, device=DEV)
+    from csaq.kvcache import KVWorkspace
+    out = c.attend(q, at, workspace=KVWorkspace(torch.zeros(Hkv * 600 * (D + 2), device=DEV))).view(Hkv, D)
+    assert torch.equal(out, c.attend(q, at).view(Hkv, D))
+    kk, vv = (t[0, :, L - n:].double() for t in c.read(0, L, dtype=torch.float32))
+    s = torch.einsum("hd,hnd->hn", q.double().view(Hkv, D), kk) * D ** -0.5
+    w = s.exp() / (s.exp().sum(1, keepdim=True) + (L - n))  # the zero keys have score 0 and value 0
+    want, mag = torch.einsum("hn,hnd->hd", w, vv), torch.einsum("hn,hnd->hd", w, vv.abs())
+    # roundings of the output (2^-25 below the normal numbers), of each weight times its
+    # value's scale, and the scores' own
+    tol = 2.0 ** -11 * want.abs() + 2.0 ** -25 + (2.0 ** -11 + 2.0 ** -12) * mag
+    assert ((out.double() - want).abs() <= tol).all()
+
+
 def test_decode_loop_captured():
     """Prompt, then steps of write + attend as one captured graph, against 64-bit
     attention over everything written; another stream with its own workspace
