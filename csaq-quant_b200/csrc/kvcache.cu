@@ -1281,10 +1281,11 @@ struct LaunchRead {
 };
 
 // How a cache is cut into chunks, from B * Hkv, Lmax and the bits alone (so that a step's token
-// count does not move the borders). Up to 8 chunks a head are the CTAs of a cluster,
-// fewer when the heads alone are four CTAs for every place on the SMs (chunks even out
-// unequal lengths: 32 sequences x 8 heads of up to 8192 keys, 8-bit, take 60 us in 8
-// chunks, 67 in 2). Where 8 leave SMs without a CTA and the cache is long, one wave
+// count does not move the borders). Up to 8 chunks a head are the CTAs of a cluster: as
+// many as one wave takes, and of kEven keys and more up to four waves of them, which even
+// out unequal lengths: 32 x 8 heads, 8-bit, of up to 8192 keys take 57 us in 6 chunks, 60
+// in 8 and 67 in 2, of up to 32768 198 in 8, 211 in 6 and 245 in 2, of up to 1024 14 in 2 and
+// 20 in 8. Where 8 leave SMs without a CTA and the cache is long, one wave
 // of CTAs leaves partials: 1 x 8 heads x 131072 keys, 8-bit, 58 us against 117; at
 // 8192 keys the second kernel costs what the wave gains (11.6 and 11.1 us). 4-bit codes,
 // bound by instructions, gain from a full wave at up to 73 heads, too, once they are long:
@@ -1295,12 +1296,12 @@ struct Split {
   bool partial;
 };
 constexpr int64_t kSms = 148, kSlots = 4 * kSms;  // CTAs that run at once (one row block of up to 8 rows)
+constexpr int64_t kEven = 1280;
 Split split_of(int64_t heads, int64_t Lmax, int bits) {
   Split s;
   s.partial = heads * kMaxCluster < kSms ? Lmax > 8192 : bits == 4 && heads * kMaxCluster < kSlots && Lmax > 16384;
-  int64_t n = s.partial ? kSlots / heads : 4 * kSlots / heads;
-  if (!s.partial && n > kMaxCluster) n = kMaxCluster;
-  if (n < 1) n = 1;
+  int64_t n = std::max<int64_t>(kSlots / heads, 1);
+  if (!s.partial) n = std::min<int64_t>(kMaxCluster, std::max(n, std::min(4 * kSlots / heads, Lmax / kEven)));
   s.chunk = (int)(((Lmax + n - 1) / n + kStep - 1) / kStep * kStep);
   s.n = (int)((Lmax + s.chunk - 1) / s.chunk);
   return s;
