@@ -351,9 +351,10 @@ __global__ void __launch_bounds__(256) kvq_read_kernel(const uint8_t* __restrict
 // result does not depend on how many tokens share its step.
 //
 // Bound by HBM for 8 bits (4 x 8 heads x 65536 keys of 128: 94 us, 0.90 of the measured
-// copy rate), by instruction issue for 4 (8 x 8 x 65536: 134 us, 0.69 of it: half the
+// copy rate), by instruction issue for 4 (8 x 8 x 65536: 124 us, 0.75 of it: half the
 // bytes, the same operands to build, about 340 instructions for 16 keys); the smallest
-// calls by one chain of latencies (1 x 8 heads x 517 keys: 4.9 us).
+// calls by one chain of latencies (1 x 8 heads x 517 keys: 4.9 us), and many rows by
+// operands and registers (4 x 8 heads x 4101 keys, 20 rows: 19 us).
 constexpr int kWarps = 4;
 constexpr int kTile = 16;
 constexpr int kStep = kWarps * 2 * kTile;  // keys that a CTA's warps take in turn
@@ -1296,7 +1297,7 @@ struct Split {
   bool partial;
 };
 constexpr int64_t kSms = 148, kSlots = 4 * kSms;  // CTAs that run at once (one row block of up to 8 rows)
-constexpr int64_t kEven = 1280;
+constexpr int64_t kEven = 1280;  // keys of a chunk that only evens out lengths
 Split split_of(int64_t heads, int64_t Lmax, int bits) {
   Split s;
   s.partial = heads * kMaxCluster < kSms ? Lmax > 8192 : bits == 4 && heads * kMaxCluster < kSlots && Lmax > 16384;
@@ -1362,11 +1363,11 @@ struct LaunchAttn {
   int run() const {
     const int64_t R = (int64_t)a.S * (a.Hq / a.Hkv);
     // Rows of a CTA: all of them while that is 24, since each block of rows builds its
-    // operands from the codes anew (16 x 8 heads x 4096 keys, 20 rows: 64 us with 24, 83 with
-    // two blocks of 16, 80 with three of 8), and 16 from then on (16 x 8 x 8192, 32 rows:
-    // 133 us with 16, 181 with 24, 202 with 32, which the registers hold once an SM).
-    // Blocks of 8 when all CTAs then run at once: few CTAs wait for latency (8 heads x 4101
-    // keys, 20 rows: 11.2 us with 8, 14.8 with 24; x 2048, 64 rows: 10.8 with 8, 12.3 with 16).
+    // operands from the codes anew (16 x 8 heads x 4096 keys, 20 rows: 48 us with 24, 64 with
+    // two blocks of 16, 69 with three of 8), and 16 from then on (16 x 8 x 8192, 32 rows:
+    // 114 us with 16, 160 with 24, which run twice an SM).
+    // Blocks of 8 when all CTAs then run at once: few CTAs wait for latency (8 heads x 4096
+    // keys, 20 rows: 10.0 us with 8, 13.1 with 24; x 2048, 64 rows: 10.3 with 8, 12.0 with 16).
     if (R <= 8 || B * a.Hkv * split.n * ((R + 7) / 8) <= kSlots) return go<BITS, D, G, 1>();
     return R <= 16 || R > 24 ? go<BITS, D, G, 2>() : go<BITS, D, G, 3>();
   }

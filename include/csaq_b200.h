@@ -464,8 +464,8 @@ int csaq_sample_rows(const void* logits, int n_parts, int64_t part_stride, int64
                      int dtype, void* stream);
 /* Sampling settings of csaq_sample_filtered: a device array of one value per
  * row, or (pointer null) one value for all rows. temperature not above 0: the
- * first rank; outside [1e-30, 1e30]: the nearer of the two; top_k <= 0, top_p >= 1 (or NaN) and min_p <= 0 (or NaN) are off;
- * top_p <= 0 keeps the first rank. */
+ * first rank; outside [1e-30, 1e30]: the nearer of the two; top_k <= 0, top_p >= 1
+ * (or NaN) and min_p <= 0 (or NaN) are off; top_p <= 0 keeps the first rank. */
 typedef struct csaq_sample_params {
   const float* temperature;
   const int32_t* top_k;
@@ -484,7 +484,8 @@ typedef struct csaq_sample_params {
  * those the ranks whose preceding mass is at most top_p times the mass of the
  * top-k set; min-p keeps of those the tokens with w_j >= min_p. out[row] is the
  * first index whose cumulative kept weight, in index order, exceeds random[row]
- * times the kept mass. Sums are fp64 in a fixed order, weights good to 2^-32. NaN
+ * times the kept mass. Sums are fp64 in a fixed order, weights good to 2^-32; those
+ * under e^-50 count as 0. NaN
  * and -inf logits are never drawn, +inf ones share the whole mass; a row of NaN
  * and -inf gives -1. Rows are n_parts slices like csaq_sample_rows; a row of
  * up to 340,000 fp32 or 680,000 16-bit logits (else CSAQ_ERR_UNSUPPORTED). */
