@@ -810,6 +810,7 @@ class DecodeRuntime:
         params = sample_params(self.B, self.dev, **self.settings)
         check(L.csaq_sample_filtered(src, n_parts, pstride, ld, plen, self.B, ctypes.byref(params),
                                      self.rand.data_ptr(), self.argmax_buf.data_ptr(), self.dt, st), "sample_filtered")
+        self.argmax_buf[: self.B].clamp_(min=0)  # -1, nothing to draw, is no row of the embedding
         check(L.csaq_greedy_commit(self.argmax_buf.data_ptr(), self.B, self.pos0.data_ptr(),
                                    self.out_tokens.data_ptr(), self.n_out.data_ptr(), self.cap,
                                    self.next_tok.data_ptr(), self.remaining.data_ptr(), st), "commit")
@@ -820,13 +821,16 @@ class DecodeRuntime:
         """Decode after reset(), one token per step, drawn by the caller's numbers:
         random[b, i] in [0, 1) draws token i of sequence b (token 0 from the
         prefill's logits). The settings are numbers or one value per sequence
-        (csaq.sampling.sample_tokens). Returns the steps run."""
+        (csaq.sampling.sample_tokens); logits that hold nothing to draw (NaN)
+        give token 0. Returns the steps run."""
         B = self.B
         if random.dim() != 2 or random.shape[0] != B or random.shape[1] < 1 or not random.is_floating_point():
             raise ValueError(f"random must hold ({B}, tokens) numbers, got {tuple(random.shape)} {random.dtype}")
         # the state must have room for the tokens: reset() set max_new
         n = random.shape[1]
         room = int(self.remaining.max()) + 1
+        if not hasattr(self, "prefill_logits") or int(self.n_out.max()) != 1:
+            raise RuntimeError("generate_sampled follows reset(), and draws all of its tokens")
         if n > room:
             raise ValueError(f"{n} random numbers for {room} tokens (max_new of reset)")
         given = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
@@ -839,10 +843,9 @@ class DecodeRuntime:
             else:
                 self.settings[k].fill_(v)
         numbers = random.to(device=self.dev, dtype=torch.float32).t().contiguous()
-        if not hasattr(self, "prefill_logits"):
-            raise RuntimeError("generate_sampled follows reset()")
         self.rand.copy_(numbers[0])
         sample_tokens(self.prefill_logits, self.rand, **self.settings, out=self.next_tok)
+        self.next_tok.clamp_(min=0)
         self.out_tokens[:, 0] = self.next_tok
         if n > 1:
             g = self._graph("sampled_v" if verify else "sampled_d", lambda: self._sampled_step(verify))

@@ -173,6 +173,31 @@ def test_one_number_draws_the_prefill_token(models):
                                                 temperature=0.7, top_k=5)[0]
 
 
+def test_steps_with_nothing_to_draw(models):
+    """Logits of NaN: token 0, a row of the embedding, in the prefill's draw and the steps'."""
+    eng = _engine(models, "tiny-llama", kv_bits=8)
+    prompt, u = _prompt(2, 9, eng.model.config.vocab_size, seed=8), torch.full((2, 5), 0.5)
+    want, _ = eng.generate(prompt, max_new_tokens=5, random=u)
+    norm = eng.model.model.norm.weight.data
+    kept = norm.clone()
+    norm.fill_(float("nan"))
+    try:
+        out, _ = eng.generate(prompt, max_new_tokens=5, random=u)
+    finally:
+        norm.copy_(kept)
+    assert (out[:, 9:] == 0).all() and torch.equal(out[:, :9], prompt)
+    assert torch.equal(eng.generate(prompt, max_new_tokens=5, random=u)[0], want)
+
+
+def test_tokens_are_drawn_once_after_a_reset(models):
+    eng = _engine(models, "tiny-llama", kv_bits=8)
+    rt = eng.runtime(1, 64, 1)
+    rt.reset(_prompt(1, 6, eng.model.config.vocab_size, seed=1).to(DEV), 8)
+    assert rt.generate_sampled(torch.full((1, 3), 0.5)) == 2
+    with pytest.raises(RuntimeError, match="reset"):
+        rt.generate_sampled(torch.full((1, 3), 0.5))
+
+
 def test_kernel_counts_follow_the_cache(models):
     a, b = _engine(models, "tiny-llama"), _engine(models, "tiny-llama", kv_bits=8)
     ra, rb = a.runtime(1, 256, 4), b.runtime(1, 256, 4)
