@@ -49,7 +49,7 @@ def sample_params(rows: int, device: torch.device, temperature: Setting = 1.0, t
         raise ValueError(f"csaq-b200: top_p must be in (0, 1], got {p_all}")
     if m is None and not 0 <= m_all <= 1:
         raise ValueError(f"csaq-b200: min_p must be in [0, 1], got {m_all}")
-    return CsaqSampleParams(t, k, p, m, t_all, int(k_all), p_all, m_all)
+    return CsaqSampleParams(t, k, p, m, float(t_all), int(k_all), float(p_all), float(m_all))
 
 
 def sample_tokens(logits: torch.Tensor, random: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0,
@@ -83,6 +83,7 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, temperature: Setti
         return out
     if logits.stride(1) != 1 or logits.stride(0) < V:
         logits = logits.contiguous()
+
     def call() -> int:
         return lib().csaq_sample_filtered(logits.data_ptr(), 1, 0, logits.stride(0), V, rows, ctypes.byref(params),
                                           random.data_ptr(), out.data_ptr(), code, raw_stream(dev.index))
