@@ -194,7 +194,7 @@ class QuantizedKVCache:
             q = _rows(q)
             ldq = q.stride(0)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device \
                     or not q_out.is_contiguous():
                 raise ValueError("csaq-b200: q_out must be contiguous with q's shape and dtype")
@@ -214,8 +214,8 @@ class QuantizedKVCache:
         code = dtype_code(dtype)
         shape = (self.batch, self.kv_heads, end - start, self.head_dim)
         if out is None:
-            out = (torch.empty(shape, dtype=dtype, device=self.device),
-                   torch.empty(shape, dtype=dtype, device=self.device))
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            out = k, torch.empty_like(k)
         else:
             for t in out:
                 if tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
@@ -252,7 +252,7 @@ class QuantizedKVCache:
         at = self._positions(pos0)
         q = _rows(q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ldo = columns
         else:
             if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1 \

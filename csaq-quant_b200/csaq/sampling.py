@@ -75,7 +75,7 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, temperature: Setti
     if random.dtype != torch.float32 or random.shape != (rows,) or random.device != dev or not random.is_contiguous():
         raise ValueError(f"csaq-b200: random must be {rows} contiguous fp32 values on {dev}")
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=dev)
+        out = torch.empty_like(random, dtype=torch.int64)
     elif out.dtype != torch.int64 or out.shape != (rows,) or out.device != dev or not out.is_contiguous():
         raise ValueError(f"csaq-b200: out must be {rows} contiguous int64 values on {dev}")
     params = sample_params(rows, dev, temperature, top_k, top_p, min_p)
