@@ -54,7 +54,8 @@ constexpr double kNegligible = -50.0;  // weights under e^-50, 2e-22 of the larg
 constexpr uint32_t kAll = 0xffffffffu;
 static_assert(kBins * 2 == kWarps && kList == 4 * kThreads && kHist == 2 * kThreads, "shares of a thread");
 constexpr int kWorkBytes = kList * 8 * 2;  // two lists; or the bins of the digit passes; or copies of the histogram
-static_assert(kWorkBytes >= kBins * kThreads * 8 && kWorkBytes >= kHist * 8 * 4, "they share the work area");
+static_assert(kWorkBytes >= kBins * kThreads * 8 && kWorkBytes >= kHist * 8 * 4 && kWorkBytes >= kList * 8 + kHist * 16,
+              "they share the work area");
 
 struct FilterArgs {
   const void* logits;

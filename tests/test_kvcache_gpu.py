@@ -136,6 +136,27 @@ def test_write_edge_values(bits, D, group):
         assert grp.isnan().all(-1).sum() == 1
 
 
+@pytest.mark.parametrize("bits,D,group", LAYOUTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_write_between_two_codes(bits, D, group, dtype):
+    """Quotients on and right beside the middle between two codes, for many scales: the
+    neighbours of (i + 1/2) s in dtype, s the group's scale."""
+    n, rows = 2 ** bits - 1, 600
+    g = torch.Generator().manual_seed(17)
+    s = torch.exp2(torch.rand(rows, 1, generator=g) * 8 - 8).bfloat16().float()
+    low = torch.randint(0, n, (rows, 1), generator=g).float()  # codes from -low to n - low
+    x = (torch.randint(0, n, (rows, D), generator=g) - low + 0.5).clamp(max=n - 0.5) * s
+    x = x.to(dtype)
+    step = torch.randint(-1, 2, x.shape, generator=g, dtype=torch.int16)
+    x = (x.view(torch.int16) + step).view(dtype)
+    x[:, ::group], x[:, 1::group] = (-low * s).to(dtype), ((n - low) * s).to(dtype)
+    c = _cache(rows, 1, 16, D, bits, group)
+    c.write(x.to(DEV), x.to(DEV), torch.zeros(rows, dtype=torch.int32, device=DEV))
+    codes, words = ref.quantise(x.float().numpy(), bits, group)
+    assert np.array_equal(c.k_codes.cpu().numpy()[:, 0, 0], ref.pack(codes, bits))
+    assert np.array_equal(c.k_params.cpu().numpy()[:, 0, 0], words.view(np.int32))
+
+
 def test_write_skips_positions_outside():
     """Before 0, behind the cache and behind the tables nothing is stored; the
     queries there pass unrotated."""

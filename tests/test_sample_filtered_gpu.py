@@ -187,6 +187,29 @@ def test_crowded_cuts(dtype):
         _check(x, u, sample_tokens(x.to(DEV), u.to(DEV), **kw), **kw)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,spread,temperature", [(20011, 2.0, 1.0), (20011, 0.3, 0.5), (3001, 4.0, 2.0), (151936, 3.0, 1.0)])
+def test_the_last_kept_rank(dtype, V, spread, temperature):
+    """Rows sorted downwards, where the largest random number draws the last kept token:
+    a cut wrong by one token, or by one of its equals, shows. Cuts fall among large, small,
+    negative and subnormal logits and on both sides of zero. (A border lies within the
+    weights' 2^-32 of a bound with a chance of about 2^-32 V p per row.)"""
+    from csaq.sampling import sample_tokens
+    rows = 24
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(rows, V, generator=g) * spread).to(dtype)
+    x[rows // 2:] *= torch.logspace(0, -5, rows - rows // 2).to(dtype)[:, None]
+    x = x.sort(dim=1, descending=True).values
+    w = ((x.double() - x[:, :1].double()) / temperature).exp()
+    above = (w * (x > 0)).sum(1) / w.sum(1)  # the cut at zero
+    p = torch.linspace(0.02, 0.999, rows).double()
+    p[::3] = above[::3].clamp(0.01, 0.999)
+    u = torch.full((rows,), 1.0 - 2.0 ** -24)
+    p = p.float()
+    kw = dict(top_p=p, temperature=temperature)
+    _check(x, u, sample_tokens(x.to(DEV), u.to(DEV), top_p=p.to(DEV), temperature=temperature), **kw)
+
+
 def test_random_numbers_outside():
     """Below 0 and NaN count as 0, 1 and more as the largest number below 1."""
     from csaq.sampling import sample_tokens
