@@ -33,6 +33,11 @@
 //  none    no top-k, no top-p: the last pass alone.
 //
 // The histograms of 1/32 nat only say where to look; the answer never depends on them.
+//
+// Bound by the chain of phases between cluster barriers for few rows (1 x 128256 bf16:
+// top-k 40 12.6 us, top-p 0.9 22.8), by instruction issue and those phases for many (64 x
+// 151936: no filter 31 us, top-k 40 26, top-p 0.9 73, min-p 18, greedy 11; a copy of
+// the logits would take 3): about 80 instructions a logit for a nucleus, 45 of them the weight.
 
 #include <atomic>
 #include <cfloat>
@@ -981,16 +986,19 @@ uint32_t in = 0;  // which of the piece lie in the window
   cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
+constexpr int64_t kPlaces = 264;
 constexpr int kSmemMax = 200 * 1024;  // dynamic, beside the static struct
 
 template <typename T>
 int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
   constexpr int per = (kSmemMax - kWorkBytes) / (int)sizeof(T) / 8 * 8;
-  // CTAs of a row: as many as leave two places an SM (by shared memory), and up to 8
-  // while the rows alone leave SMs idle
+  // CTAs of a row: as few as leave two places an SM (by shared memory), since each has
+  // its share of the work between the passes (64 rows of 151936 bf16, top-p 0.9: 73 us in
+  // 5 CTAs, 80 in 8; 256 of 50257 fp32 136 in 3, 150 in 4), and up to 8 while all of them
+  // run at once (32 rows of 151936: 38 us in 8, 46 in 5). Clusters of 8 fill 264 places.
   constexpr int two = (110 * 1024 - kWorkBytes - (int)sizeof(Shared)) / (int)sizeof(T);
   int nc = 1;
-  while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * nc <= 148)) nc *= 2;
+  while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * (nc + 1) <= kPlaces)) ++nc;
   const int64_t chunk = ((a.V + nc - 1) / nc + 7) / 8 * 8;
   if (chunk > per) return CSAQ_ERR_UNSUPPORTED;
   a.chunk = (int)chunk;
