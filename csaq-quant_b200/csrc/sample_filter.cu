@@ -58,9 +58,12 @@ constexpr int kTable = 256;            // 2^(j / 256)
 constexpr double kNegligible = -50.0;  // weights under e^-50, 2e-22 of the largest, count as 0
 constexpr uint32_t kAll = 0xffffffffu;
 static_assert(kBins * 2 == kWarps && kList == 4 * kThreads && kHist == 2 * kThreads, "shares of a thread");
-constexpr int kWorkBytes = kList * 8 * 2;  // two lists; or the bins of the digit passes; or copies of the histogram
-static_assert(kWorkBytes >= kBins * kThreads * 8 && kWorkBytes >= kHist * 8 * 4 && kWorkBytes >= kList * 8 + kHist * 16,
-              "they share the work area");
+// The work area: a list, what its sort and its weights use, the histogram. Or the bins of
+// the digit passes; or, for a nucleus, copies of the histogram and then the window's keys
+// and their bins.
+constexpr int kWorkBytes = kList * 8 + kThreads * 8 + kListK * 8, kAreaBytes = kWorkBytes + kHist * 4;
+static_assert(kAreaBytes >= kBins * kThreads * 8 && kAreaBytes >= kHist * 8 * 4 && kWorkBytes >= kList * 4 + kHist * 16,
+              "they share the area");
 
 struct FilterArgs {
   const void* logits;
@@ -216,7 +219,6 @@ struct Shared {
   float wmax[kWarps];
   int pick;
   uint32_t at;
-  __align__(8) uint32_t hist[kHist];  // read by others
 };
 
 // exclusive prefix sums of N doubles a thread in thread order; the total
@@ -264,7 +266,7 @@ __device__ __forceinline__ double block_sum(double v, double* warp_sums) {
 }
 
 // Bitonic sort of n (a power of two, at most kList) in shared memory, largest first;
-// `spare` is as long. Up to a thread each they stay in registers, and neighbours up to
+// `spare` holds kThreads. Up to a thread each they stay in registers, and neighbours up to
 // 16 apart meet by shuffles.
 __device__ __forceinline__ void sort_down(uint64_t* v, uint64_t* spare, int n) {
   __syncthreads();
@@ -312,7 +314,7 @@ struct Row {
   int n;
   int64_t first;  // index of its first element
   Shared* sh;
-  uint8_t* work;  // kWorkBytes
+  uint8_t* work;  // kAreaBytes
   uint32_t rank, nc;
   int parity;
   float fmax, ch, cl, per_bin;  // largest logit, 256 / (T ln 2), bins per unit
@@ -456,7 +458,7 @@ struct Row {
   // sums do not depend on the order of the atomics.
   __device__ Cut narrow(const uint32_t* found, int n, uint32_t klo, uint32_t khi, double base, double bound) const {
     const double unit = weight(L::of_key(khi)) * 0x1p-40, per_unit = 1.0 / unit;
-    uint64_t* bins = reinterpret_cast<uint64_t*>(work + kList * 8);  // low sums of two bins, high sums of two bins
+    uint64_t* bins = reinterpret_cast<uint64_t*>(work + kList * 4);  // low sums of two bins, high sums of two bins
     Cut c{klo, base, 0.0, bound};
     for (int flip = 0;; flip ^= 1) {
       const int shift = max(0, 22 - __clz(khi - klo | 1u));
@@ -535,11 +537,12 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   const uint32_t rank = cluster_rank(), nc = cluster_size();
   const int64_t m = blockIdx.x / nc;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  T* slice = reinterpret_cast<T*>(dyn + kWorkBytes);
+  T* slice = reinterpret_cast<T*>(dyn + kAreaBytes);
   const int64_t lo = (int64_t)rank * a.chunk;
   const int n = (int)(lo >= a.V ? 0 : (a.V - lo < a.chunk ? a.V - lo : a.chunk));
   if (tid < kTable) sh.tab[tid] = exp2((double)tid / kTable);
-  for (int i = tid; i < kHist; i += kThreads) sh.hist[i] = 0;
+  uint32_t* const hist = reinterpret_cast<uint32_t*>(dyn + kWorkBytes);
+  for (int i = tid; i < kHist; i += kThreads) hist[i] = 0;
   if (tid == 0) sh.x_count = 0, sh.at = kHist, sh.x_min = kAll, sh.x_top = 0;
   pdl_wait();
   pdl_trigger();
@@ -662,10 +665,10 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
     // more when the large ones are spread over the row: a histogram of one logit a thread.
     const float u0 = tmax >= negligible ? row.depth(tmax) : (float)kHist;
     const int bin = u0 < (float)kHist ? (int)u0 : kHist;
-    if (bin < kHist) atomicAdd(&sh.hist[bin], 1u);
+    if (bin < kHist) atomicAdd(&hist[bin], 1u);
     cluster_sync();
     double v[2], before[2];
-    row.row_bins(reinterpret_cast<const uint64_t*>(sh.hist), v);
+    row.row_bins(reinterpret_cast<const uint64_t*>(hist), v);
     block_scan<2>(v, before, sh.scan);
 #pragma unroll
     for (int i = 0; i < 2; ++i)  // the bin that the k-th of them falls into
@@ -691,7 +694,7 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
 #pragma unroll
           for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < m1 ? row.weight(Row<T>::logit_of(list[2 * tid + i])) : 0.0;
           const double z = block_scan<2>(w, above, sh.scan);
-          double* by_rank = reinterpret_cast<double*>(dyn) + kList;
+          double* by_rank = reinterpret_cast<double*>(dyn) + kList + kThreads;  // behind what a sort uses
           if (tid == 0) sh.at = 0;
           __syncthreads();
 #pragma unroll
@@ -705,21 +708,15 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
           __syncthreads();
           const int kept = (int)sh.at, size = pow2_from(kept);
           uint64_t mine[2];
-          double moved[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = 2 * tid + i;
             mine[i] = r < kept ? (list[r] << 32 | (uint32_t)r) : 0;  // the low half rises as the index falls
-            moved[i] = r < kept ? by_rank[r] : 0.0;
           }
           __syncthreads();
-          // weights go behind the first kListK places of the second list, which the sort uses
-          by_rank += kListK;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 2; ++i)
             if (2 * tid + i < size) list[2 * tid + i] = mine[i];
-            if (2 * tid + i < kept) by_rank[2 * tid + i] = moved[i];
-          }
           sort_down(list, list + kList, size);
 #pragma unroll
           for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < kept ? by_rank[(uint32_t)list[2 * tid + i]] : 0.0;
@@ -753,13 +750,18 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
       }
     });
     __syncthreads();
-    for (int i = tid; i < kHist; i += kThreads) {
+    uint32_t sums[2];  // (the last copies lie where the histogram goes)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = tid + j * kThreads;
       const uint4 x = reinterpret_cast<const uint4*>(copies)[2 * i], y = reinterpret_cast<const uint4*>(copies)[2 * i + 1];
-      sh.hist[i] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
+      sums[j] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
     }
+    __syncthreads();
+    hist[tid] = sums[0], hist[tid + kThreads] = sums[1];
     cluster_sync();
     double v[2], before[2];
-    row.row_bins(reinterpret_cast<const uint64_t*>(sh.hist), v);
+    row.row_bins(reinterpret_cast<const uint64_t*>(hist), v);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       v[i] *= 0x1p-15 * (double)__expf(-(float)(2 * tid + i) * (1.0f / kPerNat));
@@ -822,13 +824,12 @@ uint32_t in = 0;  // which of the piece lie in the window
           const double w = row.weight(cut), all = rint(c.mass / w), more = floor((target - c.base) / w) + 1.0;
           ties = (uint32_t)(more < all ? more : all);
           digits = false, summed = true;
-        } else {
-          cluster_sync();  // the digits take the work area that others may still read
         }
       }
     }
   }
   if (digits) {
+    cluster_sync();  // the bins take what others may still read
     uint32_t klo = L::key(fmaxf(cut, L::of_key(L::key(cut)))), alone = 0;
     const uint32_t khi = L::key(xmax);
     double alone_w = 0.0;
@@ -991,12 +992,12 @@ constexpr int kSmemMax = 200 * 1024;  // dynamic, beside the static struct
 
 template <typename T>
 int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
-  constexpr int per = (kSmemMax - kWorkBytes) / (int)sizeof(T) / 8 * 8;
+  constexpr int per = (kSmemMax - kAreaBytes) / (int)sizeof(T) / 8 * 8;
   // CTAs of a row: as few as leave two places an SM (by shared memory), since each has
   // its share of the work between the passes (64 rows of 151936 bf16, top-p 0.9: 73 us in
   // 5 CTAs, 80 in 8; 256 of 50257 fp32 136 in 3, 150 in 4), and up to 8 while all of them
   // run at once (32 rows of 151936: 38 us in 8, 46 in 5). Clusters of 8 fill 264 places.
-  constexpr int two = (110 * 1024 - kWorkBytes - (int)sizeof(Shared)) / (int)sizeof(T);
+  constexpr int two = (112 * 1024 - kAreaBytes - (int)sizeof(Shared)) / (int)sizeof(T);
   int nc = 1;
   while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * (nc + 1) <= kPlaces)) ++nc;
   const int64_t chunk = ((a.V + nc - 1) / nc + 7) / 8 * 8;
@@ -1016,7 +1017,7 @@ int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * nc));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kWorkBytes + chunk * sizeof(T);
+    cfg.dynamicSmemBytes = kAreaBytes + chunk * sizeof(T);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
