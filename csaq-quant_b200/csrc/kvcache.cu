@@ -839,14 +839,16 @@ struct WarpAttn {
     return top;
   }
   // Weights above 2^15 call for a new reference; under scales of (nearly) 0 they say
-  // nothing, and there the bound is on l.
+  // nothing, and there the bound is on l. A reference only rises: many keys under scales
+  // of 0 take l beyond its bound with weights of up to 2^87 each, and the scores that come
+  // after them may all be far lower, or masked. 2^30 such keys make 2^117, still finite.
   static constexpr float kMost = 0x1p95f;
 
   // New references for the rows whose weights call for them: each by its own weights
   // alone, whatever the other rows do.
   template <bool WHOLE, typename S>
   __device__ __forceinline__ void refer(const Tile& x, const float (&lo)[NT][2], S seen) {
-    // log2 of the values' scales; with the bound on l a sum of 2^(s - m) stays finite
+    // log2 of the values' scales, from -80 on: no weight 2^(s - m) exceeds 2^87 then
     float ea = 0.0f, eb = 0.0f;
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) ea = fmaxf(ea, word_scale(x.ua[grp])), eb = fmaxf(eb, word_scale(x.ub[grp]));
@@ -867,7 +869,7 @@ struct WarpAttn {
           high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, k));
         }
         if (call > 0.0f) {
-          const float to = high - kHead;
+          const float to = fmaxf(m[nt][j], high - kHead);
           const float f = ex2(m[nt][j] - to);  // 0 from the start
           m[nt][j] = to;
           l[nt][j] *= f;
