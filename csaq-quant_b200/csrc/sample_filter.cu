@@ -76,10 +76,12 @@ struct FilterArgs {
 };
 
 // Logits of type T as they lie in 32-bit words. Comparisons go by value: -0 and +0 are
-// one, a NaN is under everything. key(v) orders like v in as few bits as T has values.
+// one, a NaN is under everything. key(v) orders like v in as few bits as T has values;
+// T's finite values start at kLowest or above.
 template <typename T> struct Logit;
 template <> struct Logit<float> {
   static constexpr int N = 1;
+  static constexpr float kLowest = -FLT_MAX;
   static __device__ __forceinline__ float value(uint32_t w, int) { return __uint_as_float(w); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
@@ -95,6 +97,7 @@ template <> struct Logit<float> {
 };
 template <> struct Logit<__nv_bfloat16> {
   static constexpr int N = 2;
+  static constexpr float kLowest = -FLT_MAX;
   static __device__ __forceinline__ float value(uint32_t w, int j) {
     return __uint_as_float(j ? w & 0xffff0000u : w << 16);
   }
@@ -110,6 +113,7 @@ template <> struct Logit<__nv_bfloat16> {
 };
 template <> struct Logit<__half> {
   static constexpr int N = 2;
+  static constexpr float kLowest = -65504.0f;
   static __device__ __forceinline__ float value(uint32_t w, int j) {
     return __half2float(__ushort_as_half((unsigned short)(j ? w >> 16 : w)));
   }
@@ -830,7 +834,9 @@ uint32_t in = 0;  // which of the piece lie in the window
   }
   if (digits) {
     cluster_sync();  // the bins take what others may still read
-    uint32_t klo = L::key(fmaxf(cut, L::of_key(L::key(cut)))), alone = 0;
+    // a cut below T's values (a high temperature) must not become the key of -inf, whose
+    // tokens would then be counted among the first ranks
+    uint32_t klo = L::key(fmaxf(cut, L::kLowest)), alone = 0;
     const uint32_t khi = L::key(xmax);
     double alone_w = 0.0;
     if (klo > khi) klo = khi;
