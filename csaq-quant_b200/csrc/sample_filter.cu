@@ -35,9 +35,9 @@
 // The histograms of 1/32 nat only say where to look; the answer never depends on them.
 //
 // Bound by the chain of phases between cluster barriers for few rows (1 x 128256 bf16:
-// top-k 40 12.6 us, top-p 0.9 23), by instruction issue and those phases for many (64 x
-// 151936: no filter 23 us, top-k 40 19, top-p 0.9 59, min-p 12, greedy 7.5; a copy of
-// the logits would take 3): about 80 instructions a logit for a nucleus, 45 of them the weight.
+// top-k 40 12.8 us, top-p 0.9 23), by instruction issue and those phases for many (64 x
+// 151936: no filter 26 us, top-k 40 19, top-p 0.9 64, min-p 12, greedy 7.5; a copy of
+// the logits would take 3): about 85 instructions a logit for a nucleus, 50 of them the weight.
 
 #include <atomic>
 #include <cfloat>
@@ -180,20 +180,15 @@ __device__ __forceinline__ double sum_f64(const double* p, uint32_t nc) {
 }
 
 // exp((v - x) / T) for a result of at least exp(kNegligible), with ch + cl = 256 / (T ln 2):
-// table-driven reduction (Tang 1989) in pairs of fp32. (v - x) as d + e, its product
+// table-driven reduction (Tang 1989) in pairs of fp32. (v - x) as d + e, exact; its product
 // with ch + cl as n + f with n whole; exp = 2^(n / 256) (1 + r + r^2 / 2 + r^3 / 6),
 // r = f ln 2 / 256, |r| <= 0.00136. r is good to 2^-34 and so is the bracket; fp64 takes
-// the last step alone. e is 0 for 16-bit logits unless one is under 2^-16 of the other:
-// there it is left out, 2^-25 of the larger.
-template <bool EXACT>
+// the last step alone. (e is not 0 for 16-bit logits either: those near 0 have bits below
+// an fp32 difference from the largest, and half its step over T is the weight's error.)
 __device__ __forceinline__ double exp_tab(float v, float x, float ch, float cl, const double* tab) {
-  const float d = v - x;
+  const float d = v - x, dv = d - v, e = (v - (d - dv)) - (x + dv);
   const float zh = d * ch;
-  float zl = fmaf(d, cl, fmaf(d, ch, -zh));
-  if (EXACT) {
-    const float dv = d - v;
-    zl = fmaf((v - (d - dv)) - (x + dv), ch, zl);
-  }
+  const float zl = fmaf(e, ch, fmaf(d, cl, fmaf(d, ch, -zh)));
   const float magic = 12582912.0f;  // 1.5 2^23: the sum's low bits are the rounded integer
   const float t = zh + magic;
   const int n = __float_as_int(t);  // and those of the magic number, which neither use below sees
@@ -326,7 +321,7 @@ struct Row {
   // (no branch: the weights of a piece are computed side by side; what lies under the
   // lowest logit with weight is for the caller to leave out)
   __device__ __forceinline__ double weight(float v) const {
-    return exp_tab<sizeof(T) == 4>(v, fmax, ch, cl, sh->tab);
+    return exp_tab(v, fmax, ch, cl, sh->tab);
   }
   // bins below the largest logit, in the order of the logits; kHist and more: none
   __device__ __forceinline__ float depth(float v) const { return (fmax - v) * per_bin; }
