@@ -640,9 +640,9 @@ __global__ void __launch_bounds__(kThreads) sample_filter_kernel(const FilterArg
   // The cut: logits above `cut` are kept, and the first `ties` of those at it. At first
   // it is the lowest logit with weight, or with min_p times the largest weight.
   const double limit = (double)xmax + t64 * (min_p > 0.0f ? log(fmin((double)min_p, 1.0)) : kNegligible);
-  float lowest = limit > -3.4e38 ? (float)limit : -FLT_MAX;
+  float lowest = (float)fmax(limit, -(double)FLT_MAX);
   if (min_p > 0.0f && (double)lowest < limit) lowest = nextafterf(lowest, INFINITY);
-  const float negligible = (double)xmax + t64 * kNegligible > -3.4e38 ? (float)((double)xmax + t64 * kNegligible) : -FLT_MAX;
+  const float negligible = (float)fmax((double)xmax + t64 * kNegligible, -(double)FLT_MAX);
   float cut = negligible;
   uint32_t ties = kAll;
 
