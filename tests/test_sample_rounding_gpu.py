@@ -51,3 +51,33 @@ def test_differences_of_logits_are_exact(dtype, sign, kw):
     assert torch.equal(got, torch.tensor(want)), int((got != torch.tensor(want)).sum())
     r = len(us) // 2
     assert ref.sample(x.numpy(), us[r], **kw)[0] == want[r]
+
+
+@pytest.mark.parametrize("dtype", list(LOW))
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_differences_in_a_sorted_list_are_exact(dtype, sign):
+    """The same with the first 1000 ranks alone, which are sorted and cut in one place: a border at
+    token 900, 4e-5, moves by 4e-11, ten steps of an fp32 there."""
+    from csaq.sampling import sample_tokens
+    N, top_k = 40000, 1000
+    x = torch.full((N + 1,), sign * LOW[dtype] - 40.0, dtype=torch.float64)
+    x[::100] = x[50::100] = sign * LOW[dtype]
+    x[7::200] = x[57::200] = x[107::200] = sign * LOW[dtype]
+    x[N] = 17.0
+    row = x.to(dtype)
+    low = torch.nonzero(x == sign * LOW[dtype]).view(-1)[:top_k - 1]
+    assert torch.equal(row.double()[low], x[low]) and len(low) == top_k - 1
+    w = np.exp(sign * LOW[dtype] - 17.0)
+    us, want = [], []
+    for k in range(500, 990):
+        border = k * w / (1.0 + (top_k - 1) * w)
+        below = np.float32(border)
+        below = below if float(below) < border else np.nextafter(below, np.float32(0))
+        above = np.nextafter(below, np.float32(1))
+        if min(border - float(below), float(above) - border) >= 0.1 * float(above - below):
+            us += [below, above]
+            want += [int(low[k - 1]), int(low[k])]
+    us, want = us[:256], want[:256]
+    got = sample_tokens(row.to(DEV).expand(len(us), N + 1), torch.from_numpy(np.array(us, np.float32)).to(DEV),
+                        top_k=top_k).cpu()
+    assert torch.equal(got, torch.tensor(want)), int((got != torch.tensor(want)).sum())
