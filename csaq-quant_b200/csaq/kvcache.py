@@ -262,8 +262,10 @@ class QuantizedKVCache:
         floats, part = self._floats(S, Hq), None
         if workspace is not None:
             part = workspace.part
-            if part.device != self.device or part.numel() < floats:
-                raise ValueError(f"csaq-b200: the workspace is too small for {S} tokens and {Hq} heads of this cache")
+            if part.device != self.device or part.numel() < floats or part.dtype is not torch.float32 \
+                    or not part.is_contiguous():
+                raise ValueError(f"csaq-b200: the workspace must be {floats} contiguous fp32 values on {self.device} "
+                                 f"for {S} tokens and {Hq} heads of this cache")
         elif floats:
             part = torch.empty(floats, dtype=torch.float32, device=self.device)
         self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, at, self.batch, S, Hq,
