@@ -211,6 +211,8 @@ class QuantizedKVCache:
         head_dim) in dtype (float32, float16 or bfloat16)."""
         if not 0 <= start <= end <= self.max_len:
             raise ValueError(f"csaq-b200: positions [{start}, {end}) are not inside the cache's {self.max_len}")
+        if self.device.type != "cuda":
+            raise RuntimeError(f"csaq-b200: the cache must be on a CUDA device, not {self.device}")
         code = dtype_code(dtype)
         shape = (self.batch, self.kv_heads, end - start, self.head_dim)
         if out is None:

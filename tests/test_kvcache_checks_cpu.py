@@ -30,3 +30,10 @@ def test_attend_wants_scratch_of_contiguous_floats(monkeypatch):
     for part in (torch.zeros(n), torch.zeros(n + 5), torch.zeros(2, n)):
         c.attend(q, pos0, workspace=KVWorkspace(part))
     assert launched == ["kvq_attention"] * 3
+
+
+def test_a_cache_on_the_host_cannot_be_read():
+    from csaq.kvcache import QuantizedKVCache
+    c = QuantizedKVCache(1, 1, 32, 64, bits=8, device="cpu")
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        c.read(0, 4, dtype=torch.float16)
