@@ -486,15 +486,24 @@ class DecodeRuntime:
                                sh.q_rot.data_ptr(), c._ref, self.dt, st), "kvq_write")
         if pos_host is not None and S >= PREFILL_SDPA_TOKENS:
             n = pos_host + S
-            if self.kv_read is None or self.kv_read.shape[1] < B * Hkv * n * D:
-                self.kv_read = torch.empty(2, B * Hkv * max(n, self.prefill_chunk) * D, dtype=self.dtype,
-                                           device=self.dev)
+            held = 0 if self.kv_read is None else self.kv_read.shape[1] // (B * Hkv * D)
+            if n > held:  # steps without a reset(): twofold, so that the copies left behind stay few
+                self._reserve_read_back(max(n, min(2 * held, self.Lmax)))
             k, v = (t[: B * Hkv * n * D].view(B, Hkv, n, D) for t in self.kv_read)
             check(L.csaq_kvq_read(c._ref, B, Hkv, D, 0, n, k.data_ptr(), v.data_ptr(), self.dt, st), "kvq_read")
             self._sdpa(sh, S, k, v, pos_host, scale)
             return
         check(L.csaq_kvq_attention(sh.q_rot.data_ptr(), nq, c._ref, pos.data_ptr(), B, S, Hq, Hkv, D, scale,
                                    sh.part.data_ptr(), sh.attn.data_ptr(), nq, self.dt, st), "kvq_attention")
+
+    def _reserve_read_back(self, n: int) -> None:
+        """Room for n positions of one layer's keys and values in the model's dtype. A
+        buffer that is too small goes before the larger one is allocated: grown chunk by
+        chunk, a prompt's buffers would add up to far more than the quantised cache."""
+        size = self.B * self.Hkv_l * n * self.D
+        if self.kv_read is None or self.kv_read.shape[1] < size:
+            self.kv_read = None
+            self.kv_read = torch.empty(2, size, dtype=self.dtype, device=self.dev)
 
     def _attention_launches(self) -> int:
         """Own launches of a decode step's attention: one with RoPE fused in, or
@@ -645,6 +654,8 @@ class DecodeRuntime:
         self.stats.zero_()
         prompts = prompts.to(self.dev)
         C = self.prefill_chunk
+        if self.kv_bits is not None and min(C, P) >= PREFILL_SDPA_TOKENS:
+            self._reserve_read_back(P)
         for s0 in range(0, P, C):
             chunk = prompts[:, s0:s0 + C]
             S = chunk.shape[1]
