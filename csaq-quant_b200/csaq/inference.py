@@ -246,9 +246,9 @@ class CSAQInferenceEngine:
                 and input_ids is not None and input_ids.dim() == 2 and runtime.supports(self.model))
 
     def runtime(self, batch: int, max_len: int, lookahead: int):
-        """The (cached) static decode runtime for this batch / length / lookahead."""
+        """The (cached) static decode runtime for this batch / length / lookahead and the engine's kv_bits."""
         from .runtime import DecodeRuntime
-        key = (batch, lookahead)
+        key = (batch, lookahead, self.kv_bits)
         rt = self._runtime
         if rt is None or self._runtime_key != key or rt.Lmax < max_len:
             self._runtime = None

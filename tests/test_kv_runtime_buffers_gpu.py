@@ -50,3 +50,23 @@ def test_steps_without_a_reset_get_a_buffer_too(model):
         rt.step(32, ids[s0:s0 + 32].contiguous(), rt.pos0, verify=True, last_only=True, pos_host=s0)
         sizes.append(rt.kv_read.numel())
     assert len(set(sizes)) <= 5 and max(sizes) <= 2 * rt.Hkv_l * rt.Lmax * rt.D
+
+
+def test_kv_bits_set_later_make_another_runtime(model):
+    eng = _engine(model)
+    prompt = _prompt(1, 12, eng.model.config.vocab_size, seed=1)
+    eng.generate(prompt, temperature=0.0, max_new_tokens=4)
+    assert eng._runtime.kv_bits is None
+    eng.kv_bits = 8
+    want, _ = eng.generate(prompt, temperature=0.0, max_new_tokens=4)
+    assert eng._runtime.kv_bits == 8
+    rt = eng._runtime
+    u = torch.rand(1, 4, generator=torch.Generator().manual_seed(2))
+    eng.generate(prompt, random=u, max_new_tokens=4)  # shares the runtime of one batch and cache
+    assert eng._runtime is rt
+    eng.kv_bits = None
+    eng.generate(prompt, random=u, max_new_tokens=4)
+    assert eng._runtime.kv_bits is None
+    eng.kv_bits = 5
+    with pytest.raises(ValueError, match="kv_bits"):
+        eng.generate(prompt, temperature=0.0, max_new_tokens=4)
