@@ -34,14 +34,17 @@ def cache_positions(n: int) -> int:
     return (int(n) + 15) // 16 * 16
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself when the kernels can read its rows where they are, else a copy."""
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """t and its row stride when the kernels can read its rows where they are, else a copy's."""
     ld, one = t.stride()
+    if t.shape[0] == 1:  # of a single row the stride says nothing
+        ld = t.shape[1]
     if one != 1 or ld % 8 or ld < t.shape[1] or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:  # a contiguous view at an odd offset
             t = t.clone()
-    return t
+        ld = t.shape[1]
+    return t, ld
 
 
 @dataclass
@@ -142,7 +145,7 @@ class QuantizedKVCache:
 
     def _positions(self, pos0: torch.Tensor) -> int:
         if pos0.dtype is not torch.int32 or pos0.shape != self._pos_shape or pos0.device != self.device \
-                or pos0.stride(0) != 1:
+                or not pos0.is_contiguous():
             raise ValueError(f"csaq-b200: pos0 must be {self.batch} contiguous int32 values on {self.device}")
         return pos0.data_ptr()
 
@@ -173,7 +176,7 @@ class QuantizedKVCache:
         if self._tokens(v, "v") != kind or columns != width:
             raise ValueError(f"csaq-b200: k and v must have one dtype and batch * tokens rows of {width} columns")
         at = self._positions(pos0)
-        k, v = _rows(k), _rows(v)
+        (k, ldk), (v, ldv) = _rows(k), _rows(v)
         Hq, n_rope, ldq = 0, 0, 0
         if (cos is None) != (sin is None):
             raise ValueError("csaq-b200: cos and sin come together")
@@ -191,8 +194,7 @@ class QuantizedKVCache:
             if Sq != S or code_q != code:
                 raise ValueError("csaq-b200: q must have k's rows and dtype")
             Hq = self._heads(columns)
-            q = _rows(q)
-            ldq = q.stride(0)
+            q, ldq = _rows(q)
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device \
@@ -200,8 +202,8 @@ class QuantizedKVCache:
                 raise ValueError("csaq-b200: q_out must be contiguous with q's shape and dtype")
         elif q_out is not None:
             raise ValueError("csaq-b200: q_out without q")
-        self._run(lib().csaq_kvq_write, "kvq_write", ptr(q), ldq, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-                  at, self.batch, S, Hq, self.kv_heads, self.head_dim, ptr(cos), ptr(sin), n_rope, ptr(q_out),
+        self._run(lib().csaq_kvq_write, "kvq_write", ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, at,
+                  self.batch, S, Hq, self.kv_heads, self.head_dim, ptr(cos), ptr(sin), n_rope, ptr(q_out),
                   self._ref, code)
         return q_out
 
@@ -252,15 +254,17 @@ class QuantizedKVCache:
         S, columns, code = self._tokens(q, "q")
         Hq = self._heads(columns)
         at = self._positions(pos0)
-        q = _rows(q)
+        q, ldq = _rows(q)
+        ldo = columns
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            ldo = columns
         else:
-            if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1 \
-                    or out.stride(0) < columns or out.stride(0) % 2:
+            if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1:
                 raise ValueError("csaq-b200: out must have q's shape and dtype and rows of even stride")
-            ldo = out.stride(0)
+            if out.shape[0] > 1:
+                ldo = out.stride(0)
+                if ldo < columns or ldo % 2:
+                    raise ValueError("csaq-b200: out must have q's shape and dtype and rows of even stride")
         floats, part = self._floats(S, Hq), None
         if workspace is not None:
             part = workspace.part
@@ -270,7 +274,7 @@ class QuantizedKVCache:
                                  f"for {S} tokens and {Hq} heads of this cache")
         elif floats:
             part = torch.empty(floats, dtype=torch.float32, device=self.device)
-        self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), q.stride(0), self._ref, at, self.batch, S, Hq,
+        self._run(lib().csaq_kvq_attention, "kvq_attention", q.data_ptr(), ldq, self._ref, at, self.batch, S, Hq,
                   self.kv_heads, self.head_dim, self._scale if scale is None else float(scale), ptr(part) if floats else None,
                   out.data_ptr(), ldo, code)
         return out

@@ -81,11 +81,12 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, temperature: Setti
     params = sample_params(rows, dev, temperature, top_k, top_p, min_p)
     if rows == 0:
         return out
-    if logits.stride(1) != 1 or logits.stride(0) < V:
-        logits = logits.contiguous()
+    ld = logits.stride(0) if rows > 1 else V  # of a single row the stride says nothing
+    if logits.stride(1) != 1 or ld < V:
+        logits, ld = logits.contiguous(), V
 
     def call() -> int:
-        return lib().csaq_sample_filtered(logits.data_ptr(), 1, 0, logits.stride(0), V, rows, ctypes.byref(params),
+        return lib().csaq_sample_filtered(logits.data_ptr(), 1, 0, ld, V, rows, ctypes.byref(params),
                                           random.data_ptr(), out.data_ptr(), code, raw_stream(dev.index))
 
     if dev.index == torch.cuda.current_device():
