@@ -103,6 +103,8 @@ class QuantizedKVCache:
                              f"{[tuple(t.shape) for t in (kc, kp, vc, vp)]}")
         B, Hkv, L, rowb = kc.shape
         D = rowb * 8 // bits
+        if min(B, Hkv, L) < 1:
+            raise ValueError("csaq-b200: a cache holds at least one sequence, KV head and position")
         if D not in (64, 128) or kp.shape[3] not in (1, D // 64) or L % 16:
             raise ValueError("csaq-b200: head_dim must be 64 or 128, group_size 64 or head_dim and the length a "
                              "multiple of 16")

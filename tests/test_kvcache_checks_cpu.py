@@ -37,3 +37,12 @@ def test_a_cache_on_the_host_cannot_be_read():
     c = QuantizedKVCache(1, 1, 32, 64, bits=8, device="cpu")
     with pytest.raises(RuntimeError, match="CUDA device"):
         c.read(0, 4, dtype=torch.float16)
+
+
+def test_buffers_without_a_sequence_are_refused():
+    from csaq.kvcache import QuantizedKVCache
+    z = lambda *s, t: torch.zeros(*s, dtype=t)  # noqa: E731
+    for B, H, L in ((0, 2, 16), (2, 0, 16), (2, 2, 0)):
+        with pytest.raises(ValueError):
+            QuantizedKVCache.from_buffers(z(B, H, L, 64, t=torch.uint8), z(B, H, L, 1, t=torch.int32),
+                                          z(B, H, L, 64, t=torch.uint8), z(B, H, L, 1, t=torch.int32), bits=8)
