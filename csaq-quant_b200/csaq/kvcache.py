@@ -5,7 +5,8 @@ package's own extension for long contexts and large batches: keys and values
 as 8- or 4-bit codes with one scale and zero point per (token, head, group of
 head elements), a half or a quarter of the bytes that decode attention has to
 read. ``DecodeRuntime(..., kv_bits=8)`` uses it for a whole model; the class
-below is one layer's cache for callers with a loop of their own.
+below is one layer's cache for callers with a loop of their own. It is for
+inference: no call records a gradient, whatever its inputs require.
 
 Token (b, s) of a step is row ``b*S + s`` of its matrices and sits at position
 ``pos0[b] + s``, as everywhere in the package.
@@ -251,8 +252,8 @@ class QuantizedKVCache:
                out: Optional[torch.Tensor] = None, workspace: Optional[KVWorkspace] = None) -> torch.Tensor:
         """Causal attention of a step's (rotated) queries, (B*S, heads*head_dim):
         token (b, s) attends positions 0 .. pos0[b]+s. A token at a negative
-        position sees nothing and gets zeros. scale defaults to
-        1/sqrt(head_dim). Without a workspace one is allocated for the call."""
+        position sees nothing and gets zeros. S is at most 65535. scale defaults
+        to 1/sqrt(head_dim). Without a workspace one is allocated for the call."""
         S, columns, code = self._tokens(q, "q")
         Hq = self._heads(columns)
         at = self._positions(pos0)

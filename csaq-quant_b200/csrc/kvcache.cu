@@ -147,8 +147,8 @@ __device__ __forceinline__ void load8f(const float* p, float* out) {
 // of keys and values. The next kRing heads are on their way into shared memory meanwhile;
 // each thread reads what it copied itself.
 // Bound by HBM for a prompt and by latency for a decode step. 16 x 2048 tokens of 32 + 2 x 8
-// heads of 128 (845 MB with 4-bit codes): 159 us, 5.3 TB/s; with one head a warp and its
-// loads in registers 205 us, with the division done for every code 264 us. 16 tokens: 4.4 us.
+// heads of 128 (711 MB with 4-bit codes): 131 us, 5.4 TB/s; with the division done for every
+// code 153 us. 16 tokens: 3.1 us.
 constexpr int kRing = 4, kWriteBlocks = 3;
 template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(256, kWriteBlocks) kvq_write_kernel(const WriteArgs a) {
@@ -351,10 +351,13 @@ __global__ void __launch_bounds__(256) kvq_read_kernel(const uint8_t* __restrict
 // result does not depend on how many tokens share its step.
 //
 // Bound by HBM for 8 bits (4 x 8 heads x 65536 keys of 128: 94 us, 0.90 of the measured
-// copy rate), by instruction issue for 4 (8 x 8 x 65536: 124 us, 0.75 of it: half the
-// bytes, the same operands to build, about 340 instructions for 16 keys); the smallest
-// calls by one chain of latencies (1 x 8 heads x 517 keys: 4.9 us), and many rows by
-// operands and registers (4 x 8 heads x 4101 keys, 20 rows: 19 us).
+// copy rate). 4 bits (8 x 8 x 65536: 124 us, 0.75 of it) are half the bytes with the same
+// operands to build: about 340 instructions for 16 keys, 77 us if every issue slot were
+// used, and two CTAs an SM leave half of them empty. The smallest calls are one chain of
+// latencies (1 x 8 heads x 517 keys: 4.9 us). Many rows are short of registers and of CTAs
+// (4 x 8 heads x 4101 keys, 20 rows: 19 us; of equal lengths of 2200: 17). Unequal lengths
+// cost one query row a KV head a third (16 x 16 heads of 64 in 4 bits, up to 6001 keys: 30
+// us; of equal lengths of 3190, as many keys in all: 20).
 constexpr int kWarps = 4;
 constexpr int kTile = 16;
 constexpr int kStep = kWarps * 2 * kTile;  // keys that a CTA's warps take in turn
@@ -1254,7 +1257,7 @@ struct LaunchWrite {
     constexpr int TB = 512 / D;  // tokens of a warp
     const int64_t bx = (a.M + TB - 1) / TB, by = (heads + 7) / 8;
     // heads a warp takes: one while the CTAs fit the SMs together, up to eight when there
-    // are more tokens than that (16 x 2048 tokens: 159 us with six, 179 with three)
+    // are more tokens than that (16 x 2048 tokens: 131 us with six, 152 with three)
     const int64_t each = std::max<int64_t>(1, std::min<int64_t>(8, bx * by / (148 * kWriteBlocks)));
     const dim3 grid((unsigned)bx, (unsigned)((by + each - 1) / each));
     return launch_pdl(kvq_write_kernel<T, BITS, D, G>, grid, dim3(256), 0, st, a);

@@ -35,9 +35,10 @@
 // The histograms of 1/32 nat only say where to look; the answer never depends on them.
 //
 // Bound by the chain of phases between cluster barriers for few rows (1 x 128256 bf16:
-// top-k 40 12.8 us, top-p 0.9 23), by instruction issue and those phases for many (64 x
-// 151936: no filter 26 us, top-k 40 19, top-p 0.9 64, min-p 12, greedy 7.5; a copy of
-// the logits would take 3): about 85 instructions a logit for a nucleus, 50 of them the weight.
+// top-k 40 12.8 us, top-p 0.9 23), by those phases and instruction issue for many (64 x
+// 151936: no filter 26 us, top-k 40 19, top-p 0.9 63, min-p 12, greedy 7.5; a copy of
+// the logits would take 3): about 85 instructions a logit for a nucleus, 50 of them the
+// weight, a third of its time.
 
 #include <atomic>
 #include <cfloat>
@@ -995,9 +996,9 @@ template <typename T>
 int launch_filter(FilterArgs a, int64_t rows, cudaStream_t st) {
   constexpr int per = (kSmemMax - kAreaBytes) / (int)sizeof(T) / 8 * 8;
   // CTAs of a row: as few as leave two places an SM (by shared memory), since each has
-  // its share of the work between the passes (64 rows of 151936 bf16, top-p 0.9: 59 us in
-  // 4 CTAs, 73 in 5, 80 in 8), and up to 8 while all of them run at once (32 rows of
-  // 151936: 38 us in 8, 46 in 5). Clusters of 8 fill 264 places.
+  // its share of the work between the passes (64 rows of 151936 bf16, top-p 0.9: 63 us in
+  // 4 CTAs, 75 in 5, 83 in 8), and up to 8 while all of them run at once (32 rows of
+  // 151936: 39 us in 8, 48 in 5). Clusters of 8 fill 264 places.
   constexpr int two = (112 * 1024 - kAreaBytes - (int)sizeof(Shared)) / (int)sizeof(T);
   int nc = 1;
   while (nc < kMaxCluster && ((a.V + nc - 1) / nc > two || rows * (nc + 1) <= kPlaces)) ++nc;

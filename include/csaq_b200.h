@@ -427,8 +427,10 @@ int csaq_kvq_read(const csaq_kvq_cache* cache, int64_t B, int64_t Hkv, int64_t D
 /* csaq_decode_attention against a quantised cache: token (b, s), row b*S+s of q
  * (Hq*D wide, ldq elements apart), attends keys 0 .. min(pos0[b]+s, Lmax-1); a
  * token at a negative position sees nothing and its output is 0 (an unused
- * sequence of a batch: pos0[b] = -S). Any S. q needs 16-byte alignment and ldq a
- * multiple of 8; out rows are ldo (even) elements apart. part:
+ * sequence of a batch: pos0[b] = -S). S is at most 65535. |scale| times the largest
+ * |q| must stay under 2^117 (bf16 reaches 2^128): beyond it a row
+ * may be NaN. q needs 16-byte alignment and ldq a multiple of 8; out rows are ldo
+ * (even) elements apart. part:
  * csaq_kvq_attention_workspace_floats floats of scratch (8-byte aligned; may be null
  * when that is 0; enough for either width of codes), rewritten by each call: calls
  * that may overlap on the GPU need one each. A token's result does not depend on S or on the other sequences. */
